@@ -1,6 +1,43 @@
 //! Rust binding of the B200 (sm_100a) kernels of DIAL's quantized-linear hot
 //! path: the `extern "C"` declarations of every entry point of
-//! `include/dial_cuda.h`, its `#[repr(C)]` structs, and a thin safe layer
+//! `include/dial_cuda.h`, its `/// A paged KV cache: pages `[n_pages, n_kv_heads, page_size, 128]`.
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct dial_paged_kv {
+    pub k_pages: *mut c_void,
+    pub v_pages: *mut c_void,
+    pub k_scale: *mut f32,
+    pub v_scale: *mut f32,
+    pub format: dial_kv_format,
+    pub n_kv_heads: i32,
+    pub head_dim: i32,
+    pub page_size: i32,
+    pub n_pages: i64,
+}
+
+/// Chunks of new tokens of several sequences over a paged cache.
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct dial_paged_batch {
+    pub block_table: *const i32,
+    pub kv_len: *const i32,
+    pub q_start: *const i32,
+    pub n_seqs: i32,
+    pub max_pages: i64,
+    pub max_q: i64,
+    pub max_kv: i64,
+}
+
+/// Rotary positions with 1 to 4 axes.
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct dial_rope_axes {
+    pub n_axes: i32,
+    pub section: [i32; 4],
+    pub interleaved: i32,
+}
+
+#[repr(C)]` structs, and a thin safe layer
 //! (status codes to `Result`).
 //!
 //! The reference's host side sits behind candle's `CustomOp1`
@@ -47,6 +84,11 @@ pub const DIAL_WFMT_W8A16: dial_weight_format = 0;
 pub const DIAL_WFMT_W8A16_F16S: dial_weight_format = 1;
 pub const DIAL_WFMT_Q4_0: dial_weight_format = 2;
 pub const DIAL_WFMT_Q8_0: dial_weight_format = 8;
+
+pub type dial_kv_format = i32;
+pub const DIAL_KV_F16: dial_kv_format = 1;
+pub const DIAL_KV_BF16: dial_kv_format = 2;
+pub const DIAL_KV_INT8: dial_kv_format = 3;
 
 pub type dial_stream = *mut c_void;
 
@@ -293,6 +335,25 @@ extern "C" {
                                    workspace_bytes: usize, stream: dial_stream) -> dial_status;
     pub fn dial_head_merge(keys: *const u64, n_shards: c_int, rows: i64, out_ids: *mut i32,
                            stream: dial_stream) -> dial_status;
+
+    // paged caches (no counterpart in the reference)
+    pub fn dial_paged_kv_append(qkv: *const c_void, q_norm_w: *const c_void, k_norm_w: *const c_void,
+                                cos_t: *const f32, sin_t: *const f32, table_rows: i64, positions: *const i32,
+                                axes: *const dial_rope_axes, kv: *const dial_paged_kv,
+                                batch: *const dial_paged_batch, q_out: *mut c_void, dt: dial_dtype, tokens: i64,
+                                n_heads: c_int, eps: f32, stream: dial_stream) -> dial_status;
+    pub fn dial_paged_kv_read(kv: *const dial_paged_kv, batch: *const dial_paged_batch, k_out: *mut c_void,
+                              v_out: *mut c_void, dt: dial_dtype, tokens: i64,
+                              stream: dial_stream) -> dial_status;
+    pub fn dial_paged_attention(q: *const c_void, kv: *const dial_paged_kv, batch: *const dial_paged_batch,
+                                out: *mut c_void, dt: dial_dtype, tokens: i64, n_heads: c_int, scale: f32,
+                                stream: dial_stream) -> dial_status;
+    pub fn dial_verify_drafts_workspace_bytes(rows: i64, vocab: i64) -> usize;
+    pub fn dial_verify_drafts(logits: *const c_void, dt: dial_dtype, ids: *const i32, draft_probs: *const f32,
+                              q_start: *const i32, n_seqs: c_int, temperature: *const f32, accept_u: *const f32,
+                              sample_u: *const f32, out_ids: *mut i32, n_out: *mut i32, logprobs: *mut f32,
+                              rows: i64, vocab: i64, max_q: i64, workspace: *mut c_void,
+                              workspace_bytes: usize, stream: dial_stream) -> dial_status;
 
     // stage planner (AutoPlanner::plan_with_algorithm, spm/planner.rs:378-522)
     pub fn dial_plan_stages(model: *const dial_plan_model, objective: *const dial_plan_objective,

@@ -87,6 +87,13 @@ SIGNATURES = {
     "dial_swiglu": ([_vp, _vp, _i32, _i64, _i64, _vp], _i32),
     "dial_embedding": ([_vp, _vp, _vp, _i32, _i64, _i64, _i64, _vp], _i32),
     "dial_argmax": ([_vp, _vp, _i32, _i64, _i64, _vp], _i32),
+    "dial_paged_kv_append": ([_vp, _vp, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _i32, _i64, _i32,
+                              ctypes.c_float, _vp], _i32),
+    "dial_paged_kv_read": ([_vp, _vp, _vp, _vp, _i32, _i64, _vp], _i32),
+    "dial_paged_attention": ([_vp, _vp, _vp, _vp, _i32, _i64, _i32, ctypes.c_float, _vp], _i32),
+    "dial_verify_drafts_workspace_bytes": ([_i64, _i64], _sz),
+    "dial_verify_drafts": ([_vp, _i32, _vp, _vp, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64,
+                            _vp, _sz, _vp], _i32),
     "dial_stage_comm_unique_id": ([_vp], _i32),
     "dial_stage_comm_init": ([_vp, _i32, _i32, _i32, ctypes.c_double, ctypes.POINTER(_vp)], _i32),
     "dial_stage_comm_send": ([_vp, _vp, _sz, _i32, _vp], _i32),

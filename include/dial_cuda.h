@@ -395,6 +395,131 @@ DIAL_API dial_status dial_decoder_head_shard(
 DIAL_API dial_status dial_head_merge(const uint64_t* keys, int n_shards, int64_t rows,
                                      int32_t* out_ids, dial_stream stream);
 
+/* ------------------------------------------------------------------ paged caches
+ * Serving over a paged KV cache: a chunk of new tokens of several sequences (a
+ * piece of a prompt, drafted tokens, or one token each) is appended to pages,
+ * attends over them, and drafted tokens are verified against the logits.  The
+ * reference keeps one preallocated cache per sequence (llama3/cache.rs:149-217)
+ * and has none of these; they stand next to dial_qk_norm_rope_kv_append,
+ * dial_attention and the greedy head, with the same heads (head_dim 128,
+ * n_heads % n_kv_heads == 0, at most 8 query heads per kv head).
+ *
+ * Pages are [n_pages, n_kv_heads, page_size, 128], page_size 16, 32, 64, 128 or
+ * 256, in the activations' f16 / bf16 or as int8 codes with one f32 scale per
+ * row (k_scale / v_scale [n_pages, n_kv_heads, page_size]; value = code * scale).
+ * 16-byte aligned; n_pages * n_kv_heads * page_size < 2^31.
+ */
+typedef enum {
+  DIAL_KV_F16 = 1,  /* = DIAL_F16 */
+  DIAL_KV_BF16 = 2, /* = DIAL_BF16 */
+  DIAL_KV_INT8 = 3
+} dial_kv_format;
+
+typedef struct dial_paged_kv {
+  void* k_pages;
+  void* v_pages;
+  float* k_scale; /* DIAL_KV_INT8 only */
+  float* v_scale;
+  int32_t format; /* dial_kv_format */
+  int32_t n_kv_heads;
+  int32_t head_dim; /* 128 */
+  int32_t page_size;
+  int64_t n_pages;
+} dial_paged_kv;
+
+/* A batch of chunks.  Sequence b's new tokens are rows q_start[b] .. q_start[b+1]
+ * of the token arrays and the last rows of its kv_len[b] cache rows (the new ones
+ * counted): token t has cache row kv_len[b] - (q_start[b+1] - t).  Rows of the
+ * token arrays from q_start[n_seqs] on belong to no sequence: nothing is read from
+ * or written to them.  Cache row r is row r % page_size of page
+ * block_table[b, r / page_size]; entries behind a sequence's last row are not read.
+ * A token whose cache row would be negative has none: it is not appended, reads as
+ * zeros and attends nothing (its attention is zero).  The arrays are in device
+ * memory and are checked there: a page id outside [0, n_pages), q_start that falls
+ * or passes `tokens`, a chunk longer than max_q or kv_len beyond max_pages pages
+ * sets the device error flag (DIAL_ERR_INVALID_ARG) and touches no memory outside
+ * the given arrays; that sequence's results are then unspecified. */
+typedef struct dial_paged_batch {
+  const int32_t* block_table; /* [n_seqs, max_pages] */
+  const int32_t* kv_len;      /* [n_seqs] */
+  const int32_t* q_start;     /* [n_seqs + 1] */
+  int32_t n_seqs;
+  int64_t max_pages;
+  int64_t max_q;  /* no chunk is longer */
+  int64_t max_kv; /* the longest kv_len expected (sizes the key split only) */
+} dial_paged_batch;
+
+/* Rotary positions with 1 to 4 axes (text: 1; images: time, height, width): pair i
+ * of a head (elements i, i + 64) turns by table row positions[axis(i), t].
+ * section[a] pairs belong to axis a and the sections sum to 64.  Consecutive:
+ * section[0] pairs of axis 0, then axis 1, ...; interleaved: pair i belongs to axis
+ * a = i % n_axes if i < section[a] * n_axes, else (and for a = 0) to axis 0. */
+typedef struct dial_rope_axes {
+  int32_t n_axes;
+  int32_t section[4];
+  int32_t interleaved;
+} dial_rope_axes;
+
+/* The post-QKV step over pages: split qkv [T, (Hq + 2 Hkv) * 128]; RMSNorm of each
+ * q and k head with q_norm_w / k_norm_w [128] (both NULL: none); rotary positions
+ * from cos_t / sin_t [table_rows, 64] f32 (dial_rope_tables with DIAL_F32) at
+ * positions [n_axes, T]; q goes to q_out [T, Hq, 128], k and v to the tokens' cache
+ * rows.  f32 arithmetic, one rounding to dt -- or, for DIAL_KV_INT8, scale =
+ * absmax / 127 (1 for an all-zero row) and code = round(x * (1 / scale)), halves
+ * away from zero, as dial_w8a16_quantize; a row with a NaN or an infinity is kept
+ * as NaN.  A position outside the table sets the device error flag and uses its
+ * nearest row.  Two tokens of one call must not share a cache row. */
+DIAL_API dial_status dial_paged_kv_append(
+    const void* qkv, const void* q_norm_w, const void* k_norm_w, const float* cos_t,
+    const float* sin_t, int64_t table_rows, const int32_t* positions, const dial_rope_axes* axes,
+    const dial_paged_kv* kv, const dial_paged_batch* batch, void* q_out, dial_dtype dt,
+    int64_t tokens, int n_heads, float eps, dial_stream stream);
+
+/* The batch's rows back from their pages: k_out, v_out [T, Hkv, 128] in dt (16-bit
+ * pages: the same type; int8: code * scale rounded once).  A batch whose chunks are
+ * whole sequences (q_start[b+1] - q_start[b] = kv_len[b]) reads whole caches. */
+DIAL_API dial_status dial_paged_kv_read(const dial_paged_kv* kv, const dial_paged_batch* batch,
+                                        void* k_out, void* v_out, dial_dtype dt, int64_t tokens,
+                                        dial_stream stream);
+
+/* Attention of the batch's tokens (q [T, Hq, 128] in dt) over the pages: token t
+ * attends the cache rows up to its own, out [T, Hq * 128] =
+ * softmax(scale * q.K^T) V.  Rows that a token does not attend do not touch its
+ * result, whatever they hold.  Needs no workspace. */
+DIAL_API dial_status dial_paged_attention(const void* q, const dial_paged_kv* kv,
+                                          const dial_paged_batch* batch, void* out, dial_dtype dt,
+                                          int64_t tokens, int n_heads, float scale,
+                                          dial_stream stream);
+
+/* Verification of drafted tokens.  Sequence b owns rows q_start[b] .. q_start[b+1]
+ * of logits [rows, vocab] (f32, f16 or bf16) and of ids (the chunk the target model
+ * was run on: its last accepted token, then the drafts), so row r judges draft
+ * ids[r + 1] unless it is the sequence's last.  p = softmax(logits / temperature[b]);
+ * q = row r of draft_probs [rows, vocab] (f32), or NULL: the drafts were certain.
+ * In order, a draft x is accepted if accept_u[r] * q(x) < p(x) (u in [0, 1)); at the
+ * first that is not, a token is drawn from max(p - q, 0) (p if nothing is left of
+ * it), and behind the last draft one from p: the first index whose cumulative
+ * weight exceeds sample_u[b] times the total.  temperature 0: drafts must equal the
+ * first index of the largest logit, which also is the token drawn.
+ * out_ids[r] = the token that follows row r's prefix (an accepted draft, then the
+ * drawn token), -1 behind it; n_out[b] = the number of tokens (accepted + 1; 0 for
+ * a sequence without rows); logprobs[r] (optional) = log p of it (temperature 1 for
+ * 0), 0 where out_ids is -1.  A NaN logit counts as minus infinity; of a row
+ * without any probability token 0 is drawn, with logprob -inf; an infinite logit
+ * takes all of it.  A draft outside the vocabulary is rejected.  max_q: no sequence
+ * has more rows (a longer one, or a q_start that falls or passes `rows`, sets the
+ * device error flag).  `workspace`: dial_verify_drafts_workspace_bytes(rows, vocab)
+ * bytes, 16-byte aligned, any contents; calls sharing it must not overlap. */
+DIAL_API size_t dial_verify_drafts_workspace_bytes(int64_t rows, int64_t vocab);
+DIAL_API dial_status dial_verify_drafts(const void* logits, dial_dtype dt, const int32_t* ids,
+                                        const float* draft_probs, const int32_t* q_start,
+                                        int n_seqs, const float* temperature,
+                                        const float* accept_u, const float* sample_u,
+                                        int32_t* out_ids, int32_t* n_out, float* logprobs,
+                                        int64_t rows, int64_t vocab, int64_t max_q,
+                                        void* workspace, size_t workspace_bytes,
+                                        dial_stream stream);
+
 /* ------------------------------------------------------------------ stage planner
  * Host-only (no GPU needed).  Restates AutoPlanner::plan_with_algorithm
  * (dial-core/src/spm/planner.rs:378-522, segment_cost :743-836): contiguous
