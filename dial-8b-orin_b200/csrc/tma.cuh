@@ -77,6 +77,15 @@ __device__ __forceinline__ void load_2d(uint32_t dst, const CUtensorMap* map, ui
       : "memory");
 }
 
+// 3D tiled TMA load (no multicast) completing on `bar`.
+__device__ __forceinline__ void load_3d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x,
+                                        int y, int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+      "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+
 // Starts fetching a tensor map (a __grid_constant__ kernel parameter) into the
 // TMA unit's descriptor cache, so the first copy does not wait for it.
 __device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
@@ -106,6 +115,10 @@ __device__ __forceinline__ void fence_barrier_init() {
 // SWIZZLE_128B, which need box_bytes == swizzle_bytes).
 dial_status make_byte_map(CUtensorMap* map, const void* base, int64_t rows, int64_t row_bytes,
                           int box_bytes, int box_rows, int swizzle_bytes);
+// 3D tensor map over 16-bit [tokens, heads, 128] (256-byte rows) with a {128 bytes,
+// box_heads, box_tokens} box, SWIZZLE_128B.
+dial_status make_head_map(CUtensorMap* map, const void* base, int64_t tokens, int heads, int box_heads,
+                          int box_tokens);
 
 }  // namespace tma
 }  // namespace dial
