@@ -394,15 +394,12 @@ __global__ void __launch_bounds__(Cfg<Q8>::THREADS, 1)
           }
           __syncwarp();
         }
-      }
-    } else if (warp == 10) {
-      // ------------------------------------------------ value rows behind the cache's end
-      // must not meet a zero probability as a NaN: they become zeros
-      if (!Q8 && nj > 0 && (j0 + nj) * KT > ch.kv) {
-        const int u = 2 * nj - 1, first = ch.kv - (j0 + nj - 1) * KT;
-        if (__all_sync(0xffffffffu, wait(full + 8 * (u % NS), (uint32_t)(u / NS) & 1u, err))) {
+        // value rows behind the cache's end must not meet a zero probability as a NaN: they
+        // become zeros (int8 codes are finite whatever they are)
+        const int u = 2 * nj - 1, end = ch.kv - (j0 + nj - 1) * KT;
+        if (!Q8 && end < KT && __all_sync(0xffffffffu, wait(full + 8 * (u % NS), (uint32_t)(u / NS) & 1u, err))) {
           const uint32_t slot = base + L::RING + (uint32_t)(u % NS) * SLOT;
-          for (int i = first * 8 + lane; i < KT * 8; i += 32) {
+          for (int i = end * 8 + lane; i < KT * 8; i += 32) {
             sts16(slot + i * 16, make_uint4(0, 0, 0, 0));
             sts16(slot + HALF + i * 16, make_uint4(0, 0, 0, 0));
           }

@@ -323,6 +323,8 @@ LENGTHS = [
     ([1], [1]), ([1], [2]), ([1, 1, 1], [15, 16, 17]), ([1] * 5, [127, 128, 129, 1000, 0]), ([1], [4097]),
     ([2, 5, 3], [2, 300, 1025]), ([9, 0, 1], [9, 7, 600]), ([8, 16], [8, 4000]),
     ([33], [33]), ([64, 17, 0, 1], [200, 17, 3, 900]), ([130], [130]), ([257, 3], [1300, 5]), ([40, 40], [10, 0]),
+    ([5] * 20, [1700 + 37 * b for b in range(20)]), ([1] * 20, [1701 + 37 * b for b in range(20)]),
+    ([40] * 19, [900 + 41 * b for b in range(19)]),
 ]
 
 
