@@ -6,7 +6,7 @@
 //
 // Two launches, bound by reading the logits once (and, of one row a sequence, the
 // logits again from L2 and the draft's distribution):
-//   1. every row in segments of 4096: maximum, first index of it, sum of e in f32,
+//   1. every row in segments of 1024, a warp each: maximum, first index of it, sum of e in f32,
 //      which decide the acceptances and give the log-probabilities;
 //   2. a cluster of eight CTAs per sequence joins the segments, finds the first
 //      rejected draft and draws from that row.  The index at which a cumulative sum
@@ -24,8 +24,8 @@ namespace dial {
 
 namespace {
 
-constexpr int SEG = 4096;
-constexpr int kStatThreads = 256;
+constexpr int SEG = 1024;           // a warp's piece of a row
+constexpr int kStatWarps = 4;
 constexpr int kDrawThreads = 512;
 constexpr int kWarps = kDrawThreads / 32;
 constexpr int kCluster = 8;
@@ -35,36 +35,44 @@ struct __align__(16) SegStat {
   unsigned long long key;    // argmax_key of the maximum
 };
 
-// The aligned vectors that hold elements [lo, hi) of an array of `total` elements;
-// values outside [lo, hi) and NaN come as minus infinity.
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Aligned 16-byte vectors over an array of `total` elements; a row's elements [lo, hi)
+// need not start at one.
 template <typename T>
 struct Vec {
   static constexpr int N = 16 / sizeof(T);
-  static __device__ __forceinline__ void load(const T* x, int64_t v, int64_t lo, int64_t hi, int64_t total, float (&f)[N]) {
-    const int64_t e0 = v * N;
-    if (e0 + N <= total) {
-      const uint4 u = __ldg(reinterpret_cast<const uint4*>(x) + v);
-      const T* h = reinterpret_cast<const T*>(&u);
-#pragma unroll
-      for (int i = 0; i < N; ++i) f[i] = Act<T>::to_f32(h[i]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < N; ++i) f[i] = e0 + i < total ? Act<T>::to_f32(x[e0 + i]) : 0.f;
-    }
-#pragma unroll
+  // vector v, zeros behind the array's end
+  static __device__ __forceinline__ uint4 load(const T* x, int64_t v, int64_t total) {
+    if ((v + 1) * N <= total) return __ldg(reinterpret_cast<const uint4*>(x) + v);
+    uint4 u = make_uint4(0, 0, 0, 0);
+    T* h = reinterpret_cast<T*>(&u);
     for (int i = 0; i < N; ++i)
-      if (e0 + i < lo || e0 + i >= hi || f[i] != f[i]) f[i] = -INFINITY;
+      if (v * N + i < total) h[i] = x[v * N + i];
+    return u;
+  }
+  // its values; those outside [lo, hi) and NaN as minus infinity
+  static __device__ __forceinline__ void values(uint4 u, int64_t v, int64_t lo, int64_t hi, float (&f)[N]) {
+    const T* h = reinterpret_cast<const T*>(&u);
+    const int a = (int)max(lo - v * N, (int64_t)0), b = (int)min(hi - v * N, (int64_t)N);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      f[i] = Act<T>::to_f32(h[i]);
+      if (i < a || i >= b || f[i] != f[i]) f[i] = -INFINITY;
+    }
   }
 };
 
-// exp((x - m) / T) in f32 with it = log2(e) / T, split so that the exponent is good to
-// an ulp of the result; an infinite maximum takes everything.
-__device__ __forceinline__ float weight32(float x, float m, float it, float it_lo) {
-  if (m == INFINITY) return x == m ? 1.f : 0.f;
-  if (x == -INFINITY) return 0.f;
-  const float d = x - m, h = d * it, lo = fmaf(d, it, -h) + d * it_lo;
-  return exp2f(h) * fmaf(lo, 0.6931472f, 1.f);
+// exp((x - m) / T) in f32 with it = log2(e) / T; an infinite maximum takes everything
+__device__ __forceinline__ float weight32(float x, float m, float it) {
+  if (x == m) return m == -INFINITY ? 0.f : 1.f;
+  return m == INFINITY || !(x > -INFINITY) ? 0.f : ex2((x - m) * it);
 }
+__device__ __forceinline__ float log2e_over(float temp) { return temp > 0.f ? __fdiv_rn(1.442695041f, temp) : 1.442695041f; }
 
 struct Rows {
   int64_t q0, q1;
@@ -79,15 +87,24 @@ __device__ __forceinline__ Rows rows_of(const VerifyArgs& a, int b, bool report)
 }
 
 // ------------------------------------------------------------------ 1. the rows' segments
+// Four instructions and an ex2 a value: the ex2 rate (16 a clock and SM) is what is
+// near the bytes' time.
 template <typename T>
-__global__ void __launch_bounds__(kStatThreads) verify_stats_kernel(VerifyArgs a, SegStat* __restrict__ stat) {
+__global__ void __launch_bounds__(kStatWarps * 32) verify_stats_kernel(VerifyArgs a, SegStat* __restrict__ stat, int nseg) {
   pdl_begin();
-  constexpr int N = Vec<T>::N, PER = SEG / kStatThreads / N;
-  __shared__ float red[kStatThreads / 32];
-  __shared__ unsigned long long kred[kStatThreads / 32];
-  const int nseg = (int)((a.vocab + SEG - 1) / SEG);
-  const int64_t row = blockIdx.x / nseg, total = a.rows * a.vocab;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  constexpr int N = Vec<T>::N, PER = SEG / 32 / N;
+  const int64_t w = (int64_t)blockIdx.x * kStatWarps + (threadIdx.x >> 5);
+  if (w >= a.rows * nseg) return;
+  const int64_t row = w / nseg, total = a.rows * a.vocab;
+  const int lane = threadIdx.x & 31;
+  // segments start at the row's own aligned vectors: the first has the row's first elements,
+  // the last one more vector if the row ends inside it
+  const int64_t lo = row * a.vocab, hi = lo + a.vocab;
+  const int64_t v0 = lo / N + (w - row * nseg) * (SEG / N);
+  const T* x = static_cast<const T*>(a.logits);
+  uint4 u[PER];
+#pragma unroll
+  for (int k = 0; k < PER; ++k) u[k] = Vec<T>::load(x, v0 + k * 32 + lane, total);
   int b = 0;  // the row's sequence
   for (int i = 0; i < a.n_seqs; i += 32) {
     const bool past = i + lane < a.n_seqs && __ldg(a.q_start + i + lane + 1) <= row;
@@ -96,68 +113,81 @@ __global__ void __launch_bounds__(kStatThreads) verify_stats_kernel(VerifyArgs a
     if (c < 32) break;
   }
   if (b >= a.n_seqs) return;
-  const int64_t r0 = row * a.vocab, lo = r0 + (int64_t)(blockIdx.x % nseg) * SEG;
-  const int64_t hi = min(lo + SEG, r0 + a.vocab);
-  const T* x = static_cast<const T*>(a.logits);
-  float f[PER + 1][N];  // a segment that starts inside a vector reaches into one more
-  const int64_t v0 = lo / N;
+  const float it = log2e_over(a.temperature[b]);
+  float f[PER][N], m = -INFINITY;
+  const bool inside = v0 * N >= lo && (v0 + SEG / N) * N <= hi;
 #pragma unroll
-  for (int k = 0; k < PER; ++k) Vec<T>::load(x, v0 + k * kStatThreads + threadIdx.x, lo, hi, total, f[k]);
+  for (int k = 0; k < PER; ++k) {
+    if (inside) {
+      const T* h = reinterpret_cast<const T*>(&u[k]);
 #pragma unroll
-  for (int i = 0; i < N; ++i) f[PER][i] = -INFINITY;
-  const int64_t extra = v0 + SEG / N;
-  if (threadIdx.x == 0 && extra * N < hi) Vec<T>::load(x, extra, lo, hi, total, f[PER]);
-  const float temp = a.temperature[b];
-  float m = -INFINITY;
-#pragma unroll
-  for (int k = 0; k <= PER; ++k)
-#pragma unroll
-    for (int i = 0; i < N; ++i) m = fmaxf(m, f[k][i]);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  if (lane == 0) red[warp] = m;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kStatThreads / 32; ++w) m = fmaxf(m, red[w]);
-  const double itd = (temp > 0.f ? 1.0 / (double)temp : 1.0) * 1.4426950408889634;
-  const float it = (float)itd, it_lo = (float)(itd - (double)it);
-  float s = 0.f;
-  unsigned long long key = 0ull;
-#pragma unroll
-  for (int k = 0; k <= PER; ++k)
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      s += weight32(f[k][i], m, it, it_lo);
-      if (f[k][i] == m) {
-        const int64_t e = (k < PER ? (v0 + k * kStatThreads + threadIdx.x) : extra) * N + i;
-        if (e >= lo && e < hi) key = max(key, argmax_key(m, e - r0));
-      }
+      for (int i = 0; i < N; ++i) f[k][i] = Act<T>::to_f32(h[i]);
+    } else {
+      Vec<T>::values(u[k], v0 + k * 32 + lane, lo, hi, f[k]);
     }
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    s += __shfl_xor_sync(0xffffffffu, s, o);
-    key = max(key, __shfl_xor_sync(0xffffffffu, key, o));
+    for (int i = 0; i < N; ++i) m = fmaxf(m, f[k][i]);
   }
-  __syncthreads();
-  if (lane == 0) red[warp] = s, kred[warp] = key;
-  __syncthreads();
-  if (threadIdx.x == 0) {
+  const float mine = m;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  float s = 0.f;
+  const float mt = -m * it;
+#pragma unroll
+  for (int k = 0; k < PER; ++k)
+#pragma unroll
+    for (int i = 0; i < N; ++i) s += ex2(fmaf(f[k][i], it, mt));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if (!(s < INFINITY)) {  // NaN logits, or an infinite maximum
     s = 0.f;
-    for (int w = 0; w < kStatThreads / 32; ++w) s += red[w], key = max(key, kred[w]);
-    stat[blockIdx.x] = {m, s, key};
+#pragma unroll
+    for (int k = 0; k < PER; ++k)
+#pragma unroll
+      for (int i = 0; i < N; ++i) s += weight32(f[k][i], m, it);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   }
+  unsigned long long key = 0ull;
+  if (mine == m) {
+#pragma unroll
+    for (int k = 0; k < PER; ++k)
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int64_t e = (v0 + k * 32 + lane) * N + i;
+        if (f[k][i] == m && e >= lo && e < hi) key = max(key, argmax_key(m, e - lo));
+      }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) key = max(key, __shfl_xor_sync(0xffffffffu, key, o));
+  if (lane == 0) stat[w] = {m, s, key};
 }
 
 // ------------------------------------------------------------------ 2. acceptance and the draw
+__device__ const double kPow2[64] = {
+    0x1.0000000000000p+0, 0x1.02c9a3e778061p+0, 0x1.059b0d3158574p+0, 0x1.0874518759bc8p+0,
+    0x1.0b5586cf9890fp+0, 0x1.0e3ec32d3d1a2p+0, 0x1.11301d0125b51p+0, 0x1.1429aaea92de0p+0,
+    0x1.172b83c7d517bp+0, 0x1.1a35beb6fcb75p+0, 0x1.1d4873168b9aap+0, 0x1.2063b88628cd6p+0,
+    0x1.2387a6e756238p+0, 0x1.26b4565e27cddp+0, 0x1.29e9df51fdee1p+0, 0x1.2d285a6e4030bp+0,
+    0x1.306fe0a31b715p+0, 0x1.33c08b26416ffp+0, 0x1.371a7373aa9cbp+0, 0x1.3a7db34e59ff7p+0,
+    0x1.3dea64c123422p+0, 0x1.4160a21f72e2ap+0, 0x1.44e086061892dp+0, 0x1.486a2b5c13cd0p+0,
+    0x1.4bfdad5362a27p+0, 0x1.4f9b2769d2ca7p+0, 0x1.5342b569d4f82p+0, 0x1.56f4736b527dap+0,
+    0x1.5ab07dd485429p+0, 0x1.5e76f15ad2148p+0, 0x1.6247eb03a5585p+0, 0x1.6623882552225p+0,
+    0x1.6a09e667f3bcdp+0, 0x1.6dfb23c651a2fp+0, 0x1.71f75e8ec5f74p+0, 0x1.75feb564267c9p+0,
+    0x1.7a11473eb0187p+0, 0x1.7e2f336cf4e62p+0, 0x1.82589994cce13p+0, 0x1.868d99b4492edp+0,
+    0x1.8ace5422aa0dbp+0, 0x1.8f1ae99157736p+0, 0x1.93737b0cdc5e5p+0, 0x1.97d829fde4e50p+0,
+    0x1.9c49182a3f090p+0, 0x1.a0c667b5de565p+0, 0x1.a5503b23e255dp+0, 0x1.a9e6b5579fdbfp+0,
+    0x1.ae89f995ad3adp+0, 0x1.b33a2b84f15fbp+0, 0x1.b7f76f2fb5e47p+0, 0x1.bcc1e904bc1d2p+0,
+    0x1.c199bdd85529cp+0, 0x1.c67f12e57d14bp+0, 0x1.cb720dcef9069p+0, 0x1.d072d4a07897cp+0,
+    0x1.d5818dcfba487p+0, 0x1.da9e603db3285p+0, 0x1.dfc97337b9b5fp+0, 0x1.e502ee78b3ff6p+0,
+    0x1.ea4afa2a490dap+0, 0x1.efa1bee615a27p+0, 0x1.f50765b6e4540p+0, 0x1.fa7c1819e90d8p+0};
+
 struct Exp {
   const double* table;  // 2^(j / 64)
   double m, k;          // maximum, log2(e) / T
   float mf;
   __device__ __forceinline__ double operator()(float x) const {
-    if (mf == INFINITY) return x == mf ? 1.0 : 0.0;
-    if (x == -INFINITY) return 0.0;
     const double y = ((double)x - m) * k;
-    if (y < -1000.0) return 0.0;
     const double t = fma(y, 64.0, 6755399441055744.0);  // 1.5 * 2^52: the integer in the low word
     const int n = __double2loint(t);
     const double r = fma(t - 6755399441055744.0, -1.0 / 64, y);
@@ -167,7 +197,9 @@ struct Exp {
     p = fma(p, r, 0.69314718055994530942);
     const double e = table[n & 63];
     const double v = fma(e, p * r, e);
-    return __hiloint2double(__double2hiint(v) + (n >> 6) * (1 << 20), __double2loint(v));
+    const double z = __hiloint2double(__double2hiint(v) + (n >> 6) * (1 << 20), __double2loint(v));
+    if (mf == INFINITY) return x == mf ? 1.0 : 0.0;     // an infinite maximum takes everything
+    return y > -1000.0 ? z : 0.0;                       // (minus infinity: y is not above)
   }
 };
 
@@ -185,9 +217,10 @@ __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-// The runs' sums meet: sum[w] of every CTA of the cluster; afterwards every warp
-// knows the total and, as a pair, the run that `u` times it falls in and the sum
-// before that run (the last run of any weight, should rounding leave none).
+// The runs' sums meet: sum[w] of every CTA of the cluster (a buffer that the call
+// before last used); afterwards every warp knows the total, the run that `u` times it
+// falls in and the sum before that run (the last run of any weight, should rounding
+// leave none).
 __device__ __forceinline__ double meet(double* sum, double mine, double u, int& run, double& before) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if (lane == 0) sum[warp] = mine;
@@ -226,28 +259,27 @@ __device__ __forceinline__ double meet(double* sum, double mine, double u, int& 
     run = __shfl_sync(0xffffffffu, last, l);
     before = __shfl_sync(0xffffffffu, last_before, l);
   }
-  cluster_sync();  // the sums may be written again
   return total;
 }
 
 template <typename T>
-__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kDrawThreads)
+__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kDrawThreads, 2)
     verify_draw_kernel(VerifyArgs a, const SegStat* __restrict__ stat, int nseg) {
-  pdl_begin();
-  constexpr int N = Vec<T>::N;
-  __shared__ double table[64], sum[kWarps];
-  __shared__ float row_m[kWarps];
-  __shared__ double row_z[kWarps];
-  __shared__ int row_top[kWarps], row_ok[kWarps];
+  constexpr int N = Vec<T>::N, HOLD = 40 / N;  // vectors of a run that a lane holds: 40 values
+  __shared__ double table[64], sum[2][kWarps];
+  __shared__ float row_m[kWarps], row_z[kWarps], row_x[kWarps];
+  __shared__ int row_top[kWarps], row_ok[kWarps], row_draft[kWarps];
+  pdl_trigger();
+  if (threadIdx.x < 64) table[threadIdx.x] = kPow2[threadIdx.x];
+  pdl_wait();
   const int b = blockIdx.x / kCluster, rank = blockIdx.x % kCluster;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const Rows rw = rows_of(a, b, rank == 0 && threadIdx.x == 0);
   const int64_t V = a.vocab, total = a.rows * V;
   const T* x = static_cast<const T*>(a.logits);
-  const float temp = a.temperature[b];
+  const float temp = a.temperature[b], it = log2e_over(temp);
+  const float ut = a.sample_u[b];
   const bool greedy = !(temp > 0.f);
-  const double inv_t = greedy ? 1.0 : 1.0 / (double)temp;
-  if (threadIdx.x < 64) table[threadIdx.x] = exp2((double)threadIdx.x / 64);
   if (rw.q0 == rw.q1) {
     if (rank == 0 && threadIdx.x == 0) a.n_out[b] = 0;
     return;  // the whole cluster: no rows
@@ -255,72 +287,56 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kDrawThreads)
 
   // ---- acceptance, a warp per row, sixteen rows at a time
   int64_t stop = rw.q1 - 1;
-  float m = 0.f;
-  double Z = 0.0;
-  int top = 0;
+  float m = 0.f, Z = 0.f;
+  int top = 0, draft = -1;
   bool rejected = false;
+  auto log_p = [&](float v, float mr, float z) -> float {  // log of exp((v - mr) / T) / z
+    if (z == 0.f || !(v > -INFINITY) || (mr == INFINITY && v != mr)) return -INFINITY;
+    return (v == mr ? 0.f : greedy ? v - mr : __fdiv_rn(v - mr, temp)) - logf(z);
+  };
   for (int64_t r0 = rw.q0; r0 < rw.q1; r0 += kWarps) {
     const int64_t r = r0 + warp;
     __syncthreads();
     if (r < rw.q1) {
-      float mr = -INFINITY;
+      const bool judge = r + 1 < rw.q1;
+      const int d = judge ? a.ids[r + 1] : -1;
+      const bool in = d >= 0 && d < V;
+      const float xd = in ? Act<T>::to_f32(x[r * V + d]) : -INFINITY;
+      const float qd = in && a.probs ? a.probs[r * V + d] : 1.f, ua = judge ? a.accept_u[r] : 0.f;
+      float mr = -INFINITY, z = 0.f;
       unsigned long long key = 0ull;
+#pragma unroll 4
       for (int i = lane; i < nseg; i += 32) {
         const SegStat s = stat[r * nseg + i];
-        mr = fmaxf(mr, s.m);
+        const float mn = fmaxf(mr, s.m);
+        z = z * weight32(mr, mn, it) + s.s * weight32(s.m, mn, it);
+        mr = mn;
         key = max(key, s.key);
       }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) {
-        mr = fmaxf(mr, __shfl_xor_sync(0xffffffffu, mr, o));
+        const float mo = __shfl_xor_sync(0xffffffffu, mr, o), zo = __shfl_xor_sync(0xffffffffu, z, o), mn = fmaxf(mr, mo);
+        z = z * weight32(mr, mn, it) + zo * weight32(mo, mn, it);
+        mr = mn;
         key = max(key, __shfl_xor_sync(0xffffffffu, key, o));
       }
-      double z = 0.0;
-      for (int i = lane; i < nseg; i += 32) {
-        const SegStat s = stat[r * nseg + i];
-        if (s.m == mr) z += s.s;
-        else if (mr != INFINITY && s.m != -INFINITY) z += (double)s.s * exp(((double)s.m - (double)mr) * inv_t);
-      }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
       int t = (int)(0xFFFFFFFFu - (uint32_t)key);
-      t = z == 0.0 ? 0 : (t < 0 || t >= V ? 0 : t);
-      bool ok = false;
-      if (r + 1 < rw.q1) {
-        const int draft = a.ids[r + 1];
-        ok = draft >= 0 && draft < V;
-        if (ok && greedy) {
-          ok = draft == t;
-        } else if (ok) {
-          const float xd = Act<T>::to_f32(x[r * V + draft]);
-          const double q = a.probs ? (double)a.probs[r * V + draft] : 1.0;
-          const double e = xd == mr ? (mr == -INFINITY ? 0.0 : 1.0)
-                                    : (mr == INFINITY || !(xd > -INFINITY) ? 0.0 : exp(((double)xd - (double)mr) * inv_t));
-          ok = (double)a.accept_u[r] * q * z < e;
-        }
-      }
-      if (lane == 0) row_m[warp] = mr, row_z[warp] = z, row_top[warp] = t, row_ok[warp] = ok;
+      t = z == 0.f || t < 0 || t >= V ? 0 : t;
+      const bool ok = in && (greedy ? d == t : (double)ua * qd * z < weight32(xd, mr, it));
+      if (lane == 0) row_m[warp] = mr, row_z[warp] = z, row_x[warp] = xd, row_top[warp] = t, row_ok[warp] = ok, row_draft[warp] = d;
     }
     __syncthreads();
     const int n = (int)min((int64_t)kWarps, rw.q1 - r0);
-    int k = 0;
-    while (k < n && row_ok[k]) ++k;
-    const bool done = k < n;  // row r0 + k is the last of the output: a rejected draft, or no draft left
-    auto log_p = [&](int w, float v) -> float {
-      if (row_z[w] == 0.0 || v != v) return -INFINITY;
-      if (v == row_m[w]) return (float)-log(row_z[w]);
-      return row_m[w] == INFINITY ? -INFINITY : (float)(((double)v - (double)row_m[w]) * inv_t - log(row_z[w]));
-    };
+    const unsigned good = __ballot_sync(0xffffffffu, lane < n && row_ok[lane & (kWarps - 1)]);
+    const int k = __ffs(~good) - 1;  // the accepted ones in front
     if (rank == 0 && threadIdx.x < k) {
-      const int64_t q = r0 + threadIdx.x;
-      const int draft = a.ids[q + 1];
-      a.out_ids[q] = draft;
-      if (a.logprobs) a.logprobs[q] = log_p(threadIdx.x, Act<T>::to_f32(x[q * V + draft]));
+      a.out_ids[r0 + threadIdx.x] = row_draft[threadIdx.x];
+      if (a.logprobs) a.logprobs[r0 + threadIdx.x] = log_p(row_x[threadIdx.x], row_m[threadIdx.x], row_z[threadIdx.x]);
     }
-    if (done) {
+    if (k < n) {  // row r0 + k ends the output: a rejected draft, or no draft left
       stop = r0 + k;
       rejected = stop + 1 < rw.q1;
-      m = row_m[k], Z = row_z[k], top = row_top[k];
+      m = row_m[k], Z = row_z[k], top = row_top[k], draft = row_draft[k];
       break;
     }
   }
@@ -333,124 +349,148 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kDrawThreads)
   }
   auto tell = [&](int token, float v) {
     a.out_ids[stop] = token;
-    if (!a.logprobs) return;
-    float lp = -INFINITY;
-    if (Z != 0.0 && v == m) lp = (float)-log(Z);
-    else if (Z != 0.0 && m != INFINITY && v > -INFINITY) lp = (float)(((double)v - (double)m) * inv_t - log(Z));
-    a.logprobs[stop] = lp;
+    if (a.logprobs) a.logprobs[stop] = log_p(v, m, Z);
   };
-  if (greedy || Z == 0.0) {
+  if (greedy || Z == 0.f) {
     if (rank == 0 && threadIdx.x == 0) tell(top, m);
     return;  // the whole cluster: it decides the same everywhere
   }
 
   // ---- the draw from row `stop`: run w of kCluster * kWarps, in whole vectors
-  const Exp ex{table, (double)m, inv_t * 1.4426950408889634, m};
+  const Exp ex{table, (double)m, 1.4426950408889634 / (double)temp, m};
   const int64_t lo = stop * V, hi = lo + V, v0 = lo / N, nv = (hi + N - 1) / N - v0;
   const int64_t per = (nv + kCluster * kWarps - 1) / (kCluster * kWarps);
   const int64_t a0 = v0 + min(nv, (int64_t)(rank * kWarps + warp) * per), a1 = min(v0 + nv, a0 + per);
-  const int draft = rejected ? a.ids[stop + 1] : -1;
+  uint4 held[HOLD];  // all of the run, up to 163840 values a row
+#pragma unroll
+  for (int k = 0; k < HOLD; ++k)
+    held[k] = a0 + 32 * k + lane < a1 ? Vec<T>::load(x, a0 + 32 * k + lane, total) : make_uint4(0, 0, 0, 0);
   double z64 = 0.0;
   int mode = !rejected ? 0 : (a.probs ? 2 : 1);  // all of p; p without the draft; max(p - q, 0)
-  auto weights = [&](int64_t v, double (&w)[N]) {
+  auto weights = [&](uint4 u, int64_t v, double (&w)[N]) {
     float f[N];
-    Vec<T>::load(x, v, lo, hi, total, f);
+    Vec<T>::values(u, v, lo, hi, f);
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int64_t e = v * N + i;
-      w[i] = ex(f[i]);
-      if (mode == 1 && e - lo == draft) w[i] = 0.0;
-      if (mode == 2 && e >= lo && e < hi) w[i] = fmax(fma(-(double)__ldg(a.probs + e), z64, w[i]), 0.0);
+    for (int i = 0; i < N; ++i) w[i] = ex(f[i]);
+    if (mode == 1) {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (v * N + i - lo == draft) w[i] = 0.0;
+    } else if (mode == 2) {  // times Z
+      float q[N];
+      if ((v + 1) * N <= total) {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) {
+          const float4 y = __ldg(reinterpret_cast<const float4*>(a.probs + v * N + i));
+          q[i] = y.x, q[i + 1] = y.y, q[i + 2] = y.z, q[i + 3] = y.w;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) q[i] = v * N + i < total ? a.probs[v * N + i] : 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < N; ++i)  // (outside the row w is 0 and q another row's: 0 stays)
+        w[i] = fmax(fma(-(double)q[i], z64, w[i]), 0.0);
     }
   };
   auto run_sum = [&]() {
     double s = 0.0;
-    for (int64_t v = a0 + lane; v < a1; v += 32) {
+    auto add = [&](uint4 u, int64_t v) {
       double w[N];
-      weights(v, w);
+      weights(u, v, w);
 #pragma unroll
-      for (int i = 0; i < N; ++i) s += w[i];
-    }
+      for (int i = 0; i < N; i += 2) s += w[i] + w[i + 1];
+    };
+#pragma unroll
+    for (int k = 0; k < HOLD; ++k)
+      if (a0 + 32 * k + lane < a1) add(held[k], a0 + 32 * k + lane);
+    for (int64_t v = a0 + 32 * HOLD + lane; v < a1; v += 32) add(Vec<T>::load(x, v, total), v);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
     return s;
   };
-  const double u = (double)a.sample_u[b];
+  const double u = (double)ut;
   int run;
   double before, all;
   if (mode == 2) {  // max(p - q, 0) Z = max(e - q Z, 0) with Z in f64
     mode = 0;
-    z64 = meet(sum, run_sum(), u, run, before);
+    z64 = meet(sum[1], run_sum(), u, run, before);
     mode = 2;
   }
-  all = meet(sum, run_sum(), u, run, before);
+  all = meet(sum[0], run_sum(), u, run, before);
   if (mode && !(all > 0.0)) {  // nothing left of it: from p
     mode = 0;
-    all = meet(sum, run_sum(), u, run, before);
+    all = meet(sum[1], run_sum(), u, run, before);
   }
-  if (run != rank * kWarps + warp) return;
-  const double at = u * all;
-  int token = -1;
-  double cum = before;
-  for (int64_t v = a0; v < a1; v += 32) {
-    double w[N], s = 0.0;
-    if (v + lane < a1) {
-      weights(v + lane, w);
-    } else {
+  if (run == rank * kWarps + warp) {
+    const double at = u * all;
+    int token = -1;
+    double cum = before;
+    for (int64_t v = a0; v < a1; v += 32) {
+      double w[N], s = 0.0;
+      if (v + lane < a1) {
+        weights(Vec<T>::load(x, v + lane, total), v + lane, w);
+      } else {
 #pragma unroll
-      for (int i = 0; i < N; ++i) w[i] = 0.0;
-    }
-    int last = -1;
+        for (int i = 0; i < N; ++i) w[i] = 0.0;
+      }
+      int last = -1;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      s += w[i];
-      if (w[i] > 0.0) last = i;
-    }
-    double pre = s;
+      for (int i = 0; i < N; ++i) {
+        s += w[i];
+        if (w[i] > 0.0) last = i;
+      }
+      double pre = s;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const double y = __shfl_up_sync(0xffffffffu, pre, o);
-      if (lane >= o) pre += y;
-    }
-    const double c0 = cum + (pre - s);
-    int hit = -1;
-    double c = c0;
+      for (int o = 1; o < 32; o <<= 1) {
+        const double y = __shfl_up_sync(0xffffffffu, pre, o);
+        if (lane >= o) pre += y;
+      }
+      int hit = -1;
+      double c = cum + (pre - s);
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      c += w[i];
-      if (hit < 0 && w[i] > 0.0 && c > at) hit = i;
+      for (int i = 0; i < N; ++i) {
+        c += w[i];
+        if (hit < 0 && w[i] > 0.0 && c > at) hit = i;
+      }
+      const unsigned some = __ballot_sync(0xffffffffu, hit >= 0), any = __ballot_sync(0xffffffffu, last >= 0);
+      if (some) {
+        const int l = __ffs(some) - 1;
+        token = (int)((v + l) * N + __shfl_sync(0xffffffffu, hit, l) - lo);
+        break;
+      }
+      if (any) {
+        const int l = 31 - __clz(any);
+        token = (int)((v + l) * N + __shfl_sync(0xffffffffu, last, l) - lo);
+      }
+      cum += __shfl_sync(0xffffffffu, pre, 31);
     }
-    const unsigned some = __ballot_sync(0xffffffffu, hit >= 0), any = __ballot_sync(0xffffffffu, last >= 0);
-    if (some) {
-      const int l = __ffs(some) - 1;
-      token = (int)((v + l) * N + __shfl_sync(0xffffffffu, hit, l) - lo);
-      break;
-    }
-    if (any) {
-      const int l = 31 - __clz(any);
-      token = (int)((v + l) * N + __shfl_sync(0xffffffffu, last, l) - lo);
-    }
-    cum += __shfl_sync(0xffffffffu, pre, 31);
+    token = token < 0 ? top : token;
+    if (lane == 0) tell(token, Act<T>::to_f32(x[lo + token]));
   }
-  if (lane == 0) tell(token < 0 ? top : token, Act<T>::to_f32(x[lo + (token < 0 ? top : token)]));
+  __syncwarp();
+  cluster_sync();  // nobody leaves while another reads its sums
 }
+
+// a row's vectors, from the one that holds its first element on, in pieces of SEG
+int64_t segments(int64_t vocab) { return (vocab + 7 + SEG - 1) / SEG; }
 
 }  // namespace
 
 size_t verify_workspace_bytes(int64_t rows, int64_t vocab) {
-  return (size_t)rows * ((vocab + SEG - 1) / SEG) * sizeof(SegStat);
+  return (size_t)(rows * segments(vocab)) * sizeof(SegStat);
 }
 
 template <typename T>
 static dial_status verify_t(const VerifyArgs& a, void* ws, cudaStream_t st) {
-  const int nseg = (int)((a.vocab + SEG - 1) / SEG);
+  const int64_t nseg = segments(a.vocab), blocks = (a.rows * nseg + kStatWarps - 1) / kStatWarps;
   SegStat* stat = static_cast<SegStat*>(ws);
-  if (a.rows * nseg >= (1ll << 31)) return fail(DIAL_ERR_SHAPE, "too many rows (%lld)", (long long)a.rows);
-  const dial_status s = launch_pdl("verify_stats_kernel", verify_stats_kernel<T>, dim3((unsigned)(a.rows * nseg)),
-                                   dim3(kStatThreads), 0, st, a, stat);
+  if (blocks >= (1ll << 31)) return fail(DIAL_ERR_SHAPE, "too many rows (%lld)", (long long)a.rows);
+  const dial_status s = launch_pdl("verify_stats_kernel", verify_stats_kernel<T>, dim3((unsigned)blocks),
+                                   dim3(kStatWarps * 32), 0, st, a, stat, (int)nseg);
   if (s != DIAL_OK) return s;
   return launch_pdl("verify_draw_kernel", verify_draw_kernel<T>, dim3((unsigned)a.n_seqs * kCluster), dim3(kDrawThreads), 0,
-                    st, a, stat, nseg);
+                    st, a, stat, (int)nseg);
 }
 
 dial_status launch_verify(const VerifyArgs& a, dial_dtype dt, void* ws, cudaStream_t st) {
