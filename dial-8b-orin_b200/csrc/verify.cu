@@ -32,7 +32,7 @@ constexpr int kCluster = 8;
 
 struct __align__(16) SegStat {
   float m, s;                // maximum, sum of exp((x - m) / T)
-  unsigned long long key;    // argmax_key of the maximum
+  unsigned long long key;    // argmax_key of the maximum (greedy sequences only)
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -67,11 +67,8 @@ struct Vec {
   }
 };
 
-// exp((x - m) / T) in f32 with it = log2(e) / T; an infinite maximum takes everything
-__device__ __forceinline__ float weight32(float x, float m, float it) {
-  if (x == m) return m == -INFINITY ? 0.f : 1.f;
-  return m == INFINITY || !(x > -INFINITY) ? 0.f : ex2((x - m) * it);
-}
+// exp((x - m) / T) in f32 with it = log2(e) / T, x <= m; an infinite maximum takes everything
+__device__ __forceinline__ float weight32(float x, float m, float it) { return x == m ? 1.f : ex2((x - m) * it); }
 __device__ __forceinline__ float log2e_over(float temp) { return temp > 0.f ? __fdiv_rn(1.442695041f, temp) : 1.442695041f; }
 
 struct Rows {
@@ -113,7 +110,7 @@ __global__ void __launch_bounds__(kStatWarps * 32) verify_stats_kernel(VerifyArg
     if (c < 32) break;
   }
   if (b >= a.n_seqs) return;
-  const float it = log2e_over(a.temperature[b]);
+  const float temp = a.temperature[b], it = log2e_over(temp);
   float f[PER][N], m = -INFINITY;
   const bool inside = v0 * N >= lo && (v0 + SEG / N) * N <= hi;
 #pragma unroll
@@ -139,27 +136,30 @@ __global__ void __launch_bounds__(kStatWarps * 32) verify_stats_kernel(VerifyArg
     for (int i = 0; i < N; ++i) s += ex2(fmaf(f[k][i], it, mt));
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  if (!(s < INFINITY)) {  // NaN logits, or an infinite maximum
+  if (!(s < INFINITY)) {  // NaN logits, an infinite maximum, or none
     s = 0.f;
 #pragma unroll
     for (int k = 0; k < PER; ++k)
 #pragma unroll
-      for (int i = 0; i < N; ++i) s += weight32(f[k][i], m, it);
+      for (int i = 0; i < N; ++i)
+        if (f[k][i] > -INFINITY) s += weight32(f[k][i], m, it);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   }
   unsigned long long key = 0ull;
-  if (mine == m) {
+  if (!(temp > 0.f)) {  // greedy: the first index of the maximum
+    if (mine == m) {
+      int at = 0;
 #pragma unroll
-    for (int k = 0; k < PER; ++k)
+      for (int k = PER - 1; k >= 0; --k)
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const int64_t e = (v0 + k * 32 + lane) * N + i;
-        if (f[k][i] == m && e >= lo && e < hi) key = max(key, argmax_key(m, e - lo));
-      }
+        for (int i = N - 1; i >= 0; --i)
+          if (f[k][i] == m) at = (k * 32 + lane) * N + i;
+      key = argmax_key(m, v0 * N + at - lo);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) key = max(key, __shfl_xor_sync(0xffffffffu, key, o));
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) key = max(key, __shfl_xor_sync(0xffffffffu, key, o));
   if (lane == 0) stat[w] = {m, s, key};
 }
 
@@ -182,10 +182,10 @@ __device__ const double kPow2[64] = {
     0x1.d5818dcfba487p+0, 0x1.da9e603db3285p+0, 0x1.dfc97337b9b5fp+0, 0x1.e502ee78b3ff6p+0,
     0x1.ea4afa2a490dap+0, 0x1.efa1bee615a27p+0, 0x1.f50765b6e4540p+0, 0x1.fa7c1819e90d8p+0};
 
+// exp((x - m) / T), x <= m finite or minus infinity
 struct Exp {
   const double* table;  // 2^(j / 64)
   double m, k;          // maximum, log2(e) / T
-  float mf;
   __device__ __forceinline__ double operator()(float x) const {
     const double y = ((double)x - m) * k;
     const double t = fma(y, 64.0, 6755399441055744.0);  // 1.5 * 2^52: the integer in the low word
@@ -198,8 +198,7 @@ struct Exp {
     const double e = table[n & 63];
     const double v = fma(e, p * r, e);
     const double z = __hiloint2double(__double2hiint(v) + (n >> 6) * (1 << 20), __double2loint(v));
-    if (mf == INFINITY) return x == mf ? 1.0 : 0.0;     // an infinite maximum takes everything
-    return y > -1000.0 ? z : 0.0;                       // (minus infinity: y is not above)
+    return y > -1000.0 ? z : 0.0;
   }
 };
 
@@ -265,8 +264,8 @@ __device__ __forceinline__ double meet(double* sum, double mine, double u, int& 
 template <typename T>
 __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kDrawThreads, 2)
     verify_draw_kernel(VerifyArgs a, const SegStat* __restrict__ stat, int nseg) {
-  constexpr int N = Vec<T>::N, HOLD = 40 / N;  // vectors of a run that a lane holds: 40 values
-  __shared__ double table[64], sum[2][kWarps];
+  constexpr int N = Vec<T>::N;
+  __shared__ double table[64], sum[2][kWarps];  // a buffer is free again two meetings later
   __shared__ float row_m[kWarps], row_z[kWarps], row_x[kWarps];
   __shared__ int row_top[kWarps], row_ok[kWarps], row_draft[kWarps];
   pdl_trigger();
@@ -322,7 +321,7 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kDrawThreads,
       }
       int t = (int)(0xFFFFFFFFu - (uint32_t)key);
       t = z == 0.f || t < 0 || t >= V ? 0 : t;
-      const bool ok = in && (greedy ? d == t : (double)ua * qd * z < weight32(xd, mr, it));
+      const bool ok = in && (greedy ? d == t : xd > -INFINITY && z > 0.f && (double)ua * qd * z < weight32(xd, mr, it));
       if (lane == 0) row_m[warp] = mr, row_z[warp] = z, row_x[warp] = xd, row_top[warp] = t, row_ok[warp] = ok, row_draft[warp] = d;
     }
     __syncthreads();
@@ -357,26 +356,30 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kDrawThreads,
   }
 
   // ---- the draw from row `stop`: run w of kCluster * kWarps, in whole vectors
-  const Exp ex{table, (double)m, 1.4426950408889634 / (double)temp, m};
+  const bool inf = m == INFINITY;  // takes everything: weights 1 at the maximum
+  const Exp ex{table, inf ? 0.0 : (double)m, 1.4426950408889634 / (double)temp};
   const int64_t lo = stop * V, hi = lo + V, v0 = lo / N, nv = (hi + N - 1) / N - v0;
   const int64_t per = (nv + kCluster * kWarps - 1) / (kCluster * kWarps);
   const int64_t a0 = v0 + min(nv, (int64_t)(rank * kWarps + warp) * per), a1 = min(v0 + nv, a0 + per);
-  uint4 held[HOLD];  // all of the run, up to 163840 values a row
-#pragma unroll
-  for (int k = 0; k < HOLD; ++k)
-    held[k] = a0 + 32 * k + lane < a1 ? Vec<T>::load(x, a0 + 32 * k + lane, total) : make_uint4(0, 0, 0, 0);
   double z64 = 0.0;
-  int mode = !rejected ? 0 : (a.probs ? 2 : 1);  // all of p; p without the draft; max(p - q, 0)
+  // 0: all of p; 1: p without the draft; 2: max(p - q, 0), after a pass for Z in f64
+  const int kind = !rejected ? 0 : (a.probs ? 2 : 1);
+  int mode = kind == 2 ? 0 : kind;
   auto weights = [&](uint4 u, int64_t v, double (&w)[N]) {
     float f[N];
     Vec<T>::values(u, v, lo, hi, f);
+    if (inf) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) f[i] = f[i] == m ? 0.f : -INFINITY;
+    }
 #pragma unroll
     for (int i = 0; i < N; ++i) w[i] = ex(f[i]);
     if (mode == 1) {
+      const int64_t at = lo + draft - v * N;
 #pragma unroll
       for (int i = 0; i < N; ++i)
-        if (v * N + i - lo == draft) w[i] = 0.0;
-    } else if (mode == 2) {  // times Z
+        if (i == at) w[i] = 0.0;
+    } else if (mode == 2) {  // max(p - q, 0) Z = max(e - q Z, 0)
       float q[N];
       if ((v + 1) * N <= total) {
 #pragma unroll
@@ -389,38 +392,37 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kDrawThreads,
         for (int i = 0; i < N; ++i) q[i] = v * N + i < total ? a.probs[v * N + i] : 0.f;
       }
 #pragma unroll
-      for (int i = 0; i < N; ++i)  // (outside the row w is 0 and q another row's: 0 stays)
+      for (int i = 0; i < N; ++i)  // (outside the row w is 0 and stays it)
         w[i] = fmax(fma(-(double)q[i], z64, w[i]), 0.0);
     }
   };
-  auto run_sum = [&]() {
+  const double u = (double)ut;
+  int run, buf = 0;
+  double before, all;
+  for (;;) {  // one copy of the sweep, for the instruction cache's sake
     double s = 0.0;
-    auto add = [&](uint4 u, int64_t v) {
+    uint4 next = a0 + lane < a1 ? Vec<T>::load(x, a0 + lane, total) : make_uint4(0, 0, 0, 0);
+#pragma unroll 1
+    for (int64_t v = a0 + lane; v < a1; v += 32) {
+      const uint4 now = next;
+      if (v + 32 < a1) next = Vec<T>::load(x, v + 32, total);
       double w[N];
-      weights(u, v, w);
+      weights(now, v, w);
 #pragma unroll
       for (int i = 0; i < N; i += 2) s += w[i] + w[i + 1];
-    };
-#pragma unroll
-    for (int k = 0; k < HOLD; ++k)
-      if (a0 + 32 * k + lane < a1) add(held[k], a0 + 32 * k + lane);
-    for (int64_t v = a0 + 32 * HOLD + lane; v < a1; v += 32) add(Vec<T>::load(x, v, total), v);
+    }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    return s;
-  };
-  const double u = (double)ut;
-  int run;
-  double before, all;
-  if (mode == 2) {  // max(p - q, 0) Z = max(e - q Z, 0) with Z in f64
-    mode = 0;
-    z64 = meet(sum[1], run_sum(), u, run, before);
-    mode = 2;
-  }
-  all = meet(sum[0], run_sum(), u, run, before);
-  if (mode && !(all > 0.0)) {  // nothing left of it: from p
-    mode = 0;
-    all = meet(sum[1], run_sum(), u, run, before);
+    all = meet(sum[buf], s, u, run, before);
+    buf ^= 1;
+    if (kind == 2 && mode == 0 && z64 == 0.0) {
+      z64 = all;
+      mode = 2;
+    } else if (mode && !(all > 0.0)) {
+      mode = 0;  // nothing left of it: from p
+    } else {
+      break;
+    }
   }
   if (run == rank * kWarps + warp) {
     const double at = u * all;
