@@ -8,11 +8,11 @@
 // logits again from L2 and the draft's distribution):
 //   1. every row in segments of 1024, a warp each: maximum, first index of it, sum of e in f32,
 //      which decide the acceptances and give the log-probabilities;
-//   2. a cluster of eight CTAs per sequence joins the segments, finds the first
+//   2. a cluster of two to eight CTAs per sequence joins the segments, finds the first
 //      rejected draft and draws from that row.  The index at which a cumulative sum
 //      over 10^5 weights passes a random number moves with its last digits, so the
-//      draw sums in f64 over exponentials good to 2^-45 (a table of 2^(j/64) and a
-//      short polynomial: P. T. P. Tang, ACM TOMS 15, 1989), eleven f64 operations a
+//      draw sums in f64 over exponentials good to 2^-34 (a table of 2^(j/64) and a
+//      short polynomial: P. T. P. Tang, ACM TOMS 15, 1989), eight f64 operations a
 //      value: every warp a run of the row, then the one run that the number falls in
 //      once more, element by element.
 #include <algorithm>
@@ -28,7 +28,6 @@ constexpr int SEG = 1024;           // a warp's piece of a row
 constexpr int kStatWarps = 4;
 constexpr int kDrawThreads = 512;
 constexpr int kWarps = kDrawThreads / 32;
-constexpr int kCluster = 8;
 
 struct __align__(16) SegStat {
   float m, s;                // maximum, sum of exp((x - m) / T)
@@ -55,9 +54,16 @@ struct Vec {
       if (v * N + i < total) h[i] = x[v * N + i];
     return u;
   }
-  // its values; those outside [lo, hi) and NaN as minus infinity
+  // its values; those outside [lo, hi) and NaN as minus infinity (NAN_STAYS: but for a
+  // vector inside, whose NaN stay)
+  template <bool NAN_STAYS>
   static __device__ __forceinline__ void values(uint4 u, int64_t v, int64_t lo, int64_t hi, float (&f)[N]) {
     const T* h = reinterpret_cast<const T*>(&u);
+    if (NAN_STAYS && v * N >= lo && (v + 1) * N <= hi) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) f[i] = Act<T>::to_f32(h[i]);
+      return;
+    }
     const int a = (int)max(lo - v * N, (int64_t)0), b = (int)min(hi - v * N, (int64_t)N);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
@@ -120,7 +126,7 @@ __global__ void __launch_bounds__(kStatWarps * 32) verify_stats_kernel(VerifyArg
 #pragma unroll
       for (int i = 0; i < N; ++i) f[k][i] = Act<T>::to_f32(h[i]);
     } else {
-      Vec<T>::values(u[k], v0 + k * 32 + lane, lo, hi, f[k]);
+      Vec<T>::template values<false>(u[k], v0 + k * 32 + lane, lo, hi, f[k]);
     }
 #pragma unroll
     for (int i = 0; i < N; ++i) m = fmaxf(m, f[k][i]);
@@ -182,23 +188,25 @@ __device__ const double kPow2[64] = {
     0x1.d5818dcfba487p+0, 0x1.da9e603db3285p+0, 0x1.dfc97337b9b5fp+0, 0x1.e502ee78b3ff6p+0,
     0x1.ea4afa2a490dap+0, 0x1.efa1bee615a27p+0, 0x1.f50765b6e4540p+0, 0x1.fa7c1819e90d8p+0};
 
-// exp((x - m) / T), x <= m finite or minus infinity
+// exp((x - m) / T) up to a factor that all of a row share, x <= m finite, minus infinity or
+// NaN (both 0), to 2^-34: eight f64 operations.  Every lane has a copy of the table in its
+// own banks: entry j of lane l at table[32 j + l].
 struct Exp {
-  const double* table;  // 2^(j / 64)
-  double m, k;          // maximum, log2(e) / T
+  const double* table;  // 2^(j / 64), this lane's
+  double k, c;          // 64 log2(e) / T, minus m times that
+  __device__ __forceinline__ Exp(const double* t, float m, double k64) : table(t + (threadIdx.x & 31)), k(k64), c(-(double)m * k64) {}
   __device__ __forceinline__ double operator()(float x) const {
-    const double y = ((double)x - m) * k;
-    const double t = fma(y, 64.0, 6755399441055744.0);  // 1.5 * 2^52: the integer in the low word
+    const double y = fma((double)x, k, c);
+    const double t = y + 6755399441055744.0;            // 1.5 * 2^52: the integer in the low word
     const int n = __double2loint(t);
-    const double r = fma(t - 6755399441055744.0, -1.0 / 64, y);
-    double p = 0.00961812910762847716;                  // ln2^j / j!
-    p = fma(p, r, 0.05550410866482157995);
-    p = fma(p, r, 0.24022650695910071233);
-    p = fma(p, r, 0.69314718055994530942);
-    const double e = table[n & 63];
+    const double r = y - (t - 6755399441055744.0);
+    double p = 2.1173137155464774e-07;                     // (ln2 / 64)^j / j!
+    p = fma(p, r, 5.864904955056169e-05);
+    p = fma(p, r, 0.010830424696249145);
+    const double e = table[(n & 63) * 32];
     const double v = fma(e, p * r, e);
     const double z = __hiloint2double(__double2hiint(v) + (n >> 6) * (1 << 20), __double2loint(v));
-    return y > -1000.0 ? z : 0.0;
+    return y > -64000.0 ? z : 0.0;
   }
 };
 
@@ -207,29 +215,31 @@ __device__ __forceinline__ uint32_t map_shared(const void* p, uint32_t rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
   return r;
 }
-__device__ __forceinline__ double ld_cluster_f64(uint32_t addr) {
-  double v;
-  asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(addr) : "memory");
-  return v;
+__device__ __forceinline__ void st_cluster_f64(uint32_t addr, double v) {
+  asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(addr), "d"(v) : "memory");
 }
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-// The runs' sums meet: sum[w] of every CTA of the cluster (a buffer that the call
-// before last used); afterwards every warp knows the total, the run that `u` times it
-// falls in and the sum before that run (the last run of any weight, should rounding
-// leave none).
-__device__ __forceinline__ double meet(double* sum, double mine, double u, int& run, double& before) {
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
+// The runs' sums meet: every warp puts its own into sum[] of every CTA of the cluster (a
+// buffer that the call before last used); afterwards every warp knows the total, the run
+// that `u` times it falls in and the sum before that run (the last run of any weight,
+// should rounding leave none).
+template <int CL>
+__device__ __forceinline__ double meet(double* sum, int rank, double mine, double u, int& run, double& before) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  if (lane == 0) sum[warp] = mine;
+  if (lane < CL) st_cluster_f64(map_shared(sum + rank * kWarps + warp, lane), mine);
+  __syncwarp();
   cluster_sync();
-  constexpr int PER = kCluster * kWarps / 32;
+  constexpr int PER = CL * kWarps / 32;
   double v[PER], s = 0.0;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
-    const int r = lane * PER + i;
-    v[i] = ld_cluster_f64(map_shared(sum + r % kWarps, r / kWarps));
+    v[i] = sum[lane * PER + i];
     s += v[i];
   }
   double pre = s;  // inclusive prefix over the lanes
@@ -240,15 +250,15 @@ __device__ __forceinline__ double meet(double* sum, double mine, double u, int& 
   }
   const double total = __shfl_sync(0xffffffffu, pre, 31), at = u * total;
   double cum = pre - s;
-  int hit = kCluster * kWarps, last = -1;
+  int hit = CL * kWarps, last = -1;
   double hit_before = 0.0, last_before = 0.0;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     if (v[i] > 0.0) last = lane * PER + i, last_before = cum;
-    if (hit == kCluster * kWarps && v[i] > 0.0 && cum + v[i] > at) hit = lane * PER + i, hit_before = cum;
+    if (hit == CL * kWarps && v[i] > 0.0 && cum + v[i] > at) hit = lane * PER + i, hit_before = cum;
     cum += v[i];
   }
-  const unsigned some = __ballot_sync(0xffffffffu, hit < kCluster * kWarps), any = __ballot_sync(0xffffffffu, last >= 0);
+  const unsigned some = __ballot_sync(0xffffffffu, hit < CL * kWarps), any = __ballot_sync(0xffffffffu, last >= 0);
   if (some) {
     const int l = __ffs(some) - 1;
     run = __shfl_sync(0xffffffffu, hit, l);
@@ -261,17 +271,19 @@ __device__ __forceinline__ double meet(double* sum, double mine, double u, int& 
   return total;
 }
 
-template <typename T>
-__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kDrawThreads, 2)
+template <typename T, int CL>
+__global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(kDrawThreads)
     verify_draw_kernel(VerifyArgs a, const SegStat* __restrict__ stat, int nseg) {
-  constexpr int N = Vec<T>::N;
-  __shared__ double table[64], sum[2][kWarps];  // a buffer is free again two meetings later
+  constexpr int N = Vec<T>::N, HOLD = 5;  // vectors of a lane whose sums are kept
+  __shared__ __align__(16) double table[64 * 32], sum[2][CL * kWarps];  // a buffer is free again two meetings later
+  __shared__ double part[HOLD][kDrawThreads];
   __shared__ float row_m[kWarps], row_z[kWarps], row_x[kWarps];
   __shared__ int row_top[kWarps], row_ok[kWarps], row_draft[kWarps];
   pdl_trigger();
-  if (threadIdx.x < 64) table[threadIdx.x] = kPow2[threadIdx.x];
+  cluster_arrive();  // every CTA runs before another writes to it
+  for (int i = threadIdx.x; i < 64 * 32; i += kDrawThreads) table[i] = kPow2[i / 32];
   pdl_wait();
-  const int b = blockIdx.x / kCluster, rank = blockIdx.x % kCluster;
+  const int b = blockIdx.x / CL, rank = blockIdx.x % CL;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const Rows rw = rows_of(a, b, rank == 0 && threadIdx.x == 0);
   const int64_t V = a.vocab, total = a.rows * V;
@@ -279,8 +291,11 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kDrawThreads,
   const float temp = a.temperature[b], it = log2e_over(temp);
   const float ut = a.sample_u[b];
   const bool greedy = !(temp > 0.f);
+  const double k64 = greedy ? 0.0 : 92.332482616893656 / (double)temp;  // 64 log2(e) / T
   if (rw.q0 == rw.q1) {
     if (rank == 0 && threadIdx.x == 0) a.n_out[b] = 0;
+    __syncwarp();
+    cluster_wait();
     return;  // the whole cluster: no rows
   }
 
@@ -352,14 +367,16 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kDrawThreads,
   };
   if (greedy || Z == 0.f) {
     if (rank == 0 && threadIdx.x == 0) tell(top, m);
+    __syncwarp();
+    cluster_wait();
     return;  // the whole cluster: it decides the same everywhere
   }
 
-  // ---- the draw from row `stop`: run w of kCluster * kWarps, in whole vectors
+  // ---- the draw from row `stop`: run w of CL * kWarps, in whole vectors
   const bool inf = m == INFINITY;  // takes everything: weights 1 at the maximum
-  const Exp ex{table, inf ? 0.0 : (double)m, 1.4426950408889634 / (double)temp};
+  const Exp ex(table, inf ? 0.f : m, k64);
   const int64_t lo = stop * V, hi = lo + V, v0 = lo / N, nv = (hi + N - 1) / N - v0;
-  const int64_t per = (nv + kCluster * kWarps - 1) / (kCluster * kWarps);
+  const int64_t per = (nv + CL * kWarps - 1) / (CL * kWarps);
   const int64_t a0 = v0 + min(nv, (int64_t)(rank * kWarps + warp) * per), a1 = min(v0 + nv, a0 + per);
   double z64 = 0.0;
   // 0: all of p; 1: p without the draft; 2: max(p - q, 0), after a pass for Z in f64
@@ -367,7 +384,7 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kDrawThreads,
   int mode = kind == 2 ? 0 : kind;
   auto weights = [&](uint4 u, int64_t v, double (&w)[N]) {
     float f[N];
-    Vec<T>::values(u, v, lo, hi, f);
+    Vec<T>::template values<true>(u, v, lo, hi, f);
     if (inf) {
 #pragma unroll
       for (int i = 0; i < N; ++i) f[i] = f[i] == m ? 0.f : -INFINITY;
@@ -396,77 +413,102 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kDrawThreads,
         w[i] = fmax(fma(-(double)q[i], z64, w[i]), 0.0);
     }
   };
+  auto weight1 = [&](int64_t e) {  // of one element of the row
+    float f = Act<T>::to_f32(x[e]);
+    if (inf) f = f == m ? 0.f : -INFINITY;
+    const double w = ex(f);
+    return mode == 1 ? (e - lo == draft ? 0.0 : w) : mode == 2 ? fmax(fma(-(double)a.probs[e], z64, w), 0.0) : w;
+  };
+  if (kind == 2)  // the draft's weights of this run, wanted after the pass for Z
+    for (int64_t e = a0 * N + 32 * lane; e < min(a1 * N, total); e += 32 * 32)
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(a.probs + e));
+  __syncwarp();
+  cluster_wait();
   const double u = (double)ut;
-  int run, buf = 0;
-  double before, all;
-  for (;;) {  // one copy of the sweep, for the instruction cache's sake
-    double s = 0.0;
-    uint4 next = a0 + lane < a1 ? Vec<T>::load(x, a0 + lane, total) : make_uint4(0, 0, 0, 0);
+  const bool single = per <= 32 * HOLD;  // all sums of the run are kept
+  int run = -1, buf = 0, token = -1;
+  double before = 0.0, all = 0.0, at = 0.0;
+  // passes over the run: for Z, for the weights, and for the place of `at`.  The loops stay
+  // rolled: code that runs once or twice a launch waits for its instructions.
+  for (;;) {
+    const bool locate = run >= 0;
+    double mine = 0.0, cum = before;
+    bool found = false;
 #pragma unroll 1
-    for (int64_t v = a0 + lane; v < a1; v += 32) {
-      const uint4 now = next;
-      if (v + 32 < a1) next = Vec<T>::load(x, v + 32, total);
-      double w[N];
-      weights(now, v, w);
+    for (int64_t c0 = a0; c0 < a1 && !found; c0 += 32 * HOLD) {
+      if (!locate || !single) {
+        uint4 next = c0 + lane < a1 ? Vec<T>::load(x, c0 + lane, total) : make_uint4(0, 0, 0, 0);
+#pragma unroll 1
+        for (int k = 0; k < HOLD; ++k) {
+          const int64_t v = c0 + 32 * k + lane;
+          const uint4 now = next;
+          if (v + 32 < a1) next = Vec<T>::load(x, v + 32, total);
+          double s = 0.0;
+          if (v < a1) {
+            double w[N];
+            weights(now, v, w);
 #pragma unroll
-      for (int i = 0; i < N; i += 2) s += w[i] + w[i + 1];
+            for (int i = 0; i < N; i += 2) s += w[i] + w[i + 1];
+          }
+          part[k][threadIdx.x] = s;
+          mine += s;
+        }
+      }
+      if (!locate) continue;
+      // the vector in which the cumulative sum passes `at`, or the last of any weight
+      int64_t vec = -1;
+      double start = 0.0;
+#pragma unroll 1
+      for (int k = 0; k < HOLD && !found; ++k) {
+        const double s = part[k][threadIdx.x];
+        double pre = s;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const double y = __shfl_up_sync(0xffffffffu, pre, o);
+          if (lane >= o) pre += y;
+        }
+        const unsigned some = __ballot_sync(0xffffffffu, s > 0.0 && cum + pre > at);
+        const unsigned any = __ballot_sync(0xffffffffu, s > 0.0);
+        if (any) {
+          const int l = some ? __ffs(some) - 1 : 31 - __clz(any);
+          vec = c0 + 32 * k + l;
+          start = cum + __shfl_sync(0xffffffffu, pre - s, l);
+          found = some != 0;
+        }
+        cum += __shfl_sync(0xffffffffu, pre, 31);
+      }
+      if (vec >= 0) {  // its element, a lane each
+        const int64_t e = vec * N + lane;
+        const double w = lane < N && e >= lo && e < hi ? weight1(e) : 0.0;
+        double pre = w;
+#pragma unroll
+        for (int o = 1; o < N; o <<= 1) {
+          const double y = __shfl_up_sync(0xffffffffu, pre, o);
+          if (lane >= o) pre += y;
+        }
+        const unsigned some = __ballot_sync(0xffffffffu, w > 0.0 && start + pre > at);
+        const unsigned any = __ballot_sync(0xffffffffu, w > 0.0);
+        token = (int)(vec * N + (some ? __ffs(some) - 1 : 31 - __clz(any)) - lo);
+      }
     }
+    if (locate) break;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    all = meet(sum[buf], s, u, run, before);
+    for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+    int r;
+    all = meet<CL>(sum[buf], rank, mine, u, r, before);
     buf ^= 1;
-    if (kind == 2 && mode == 0 && z64 == 0.0) {
+    if (kind == 2 && z64 == 0.0) {
       z64 = all;
       mode = 2;
     } else if (mode && !(all > 0.0)) {
       mode = 0;  // nothing left of it: from p
     } else {
-      break;
+      if (r != rank * kWarps + warp) break;
+      run = r;
+      at = u * all;
     }
   }
-  if (run == rank * kWarps + warp) {
-    const double at = u * all;
-    int token = -1;
-    double cum = before;
-    for (int64_t v = a0; v < a1; v += 32) {
-      double w[N], s = 0.0;
-      if (v + lane < a1) {
-        weights(Vec<T>::load(x, v + lane, total), v + lane, w);
-      } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i) w[i] = 0.0;
-      }
-      int last = -1;
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        s += w[i];
-        if (w[i] > 0.0) last = i;
-      }
-      double pre = s;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const double y = __shfl_up_sync(0xffffffffu, pre, o);
-        if (lane >= o) pre += y;
-      }
-      int hit = -1;
-      double c = cum + (pre - s);
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        c += w[i];
-        if (hit < 0 && w[i] > 0.0 && c > at) hit = i;
-      }
-      const unsigned some = __ballot_sync(0xffffffffu, hit >= 0), any = __ballot_sync(0xffffffffu, last >= 0);
-      if (some) {
-        const int l = __ffs(some) - 1;
-        token = (int)((v + l) * N + __shfl_sync(0xffffffffu, hit, l) - lo);
-        break;
-      }
-      if (any) {
-        const int l = 31 - __clz(any);
-        token = (int)((v + l) * N + __shfl_sync(0xffffffffu, last, l) - lo);
-      }
-      cum += __shfl_sync(0xffffffffu, pre, 31);
-    }
+  if (run >= 0) {
     token = token < 0 ? top : token;
     if (lane == 0) tell(token, Act<T>::to_f32(x[lo + token]));
   }
@@ -491,8 +533,13 @@ static dial_status verify_t(const VerifyArgs& a, void* ws, cudaStream_t st) {
   const dial_status s = launch_pdl("verify_stats_kernel", verify_stats_kernel<T>, dim3((unsigned)blocks),
                                    dim3(kStatWarps * 32), 0, st, a, stat, (int)nseg);
   if (s != DIAL_OK) return s;
-  return launch_pdl("verify_draw_kernel", verify_draw_kernel<T>, dim3((unsigned)a.n_seqs * kCluster), dim3(kDrawThreads), 0,
-                    st, a, stat, (int)nseg);
+  // CTAs per sequence: as many as leave every CTA an SM of its own (eight at most: the
+  // portable cluster), two from 74 sequences on
+  const int sms = sm_count();
+  const int cl = a.n_seqs * 8 <= sms ? 8 : (a.n_seqs * 4 <= sms ? 4 : 2);
+  auto k = cl == 8 ? verify_draw_kernel<T, 8> : (cl == 4 ? verify_draw_kernel<T, 4> : verify_draw_kernel<T, 2>);
+  return launch_pdl("verify_draw_kernel", k, dim3((unsigned)(a.n_seqs * cl)), dim3(kDrawThreads), 0, st, a, stat,
+                    (int)nseg);
 }
 
 dial_status launch_verify(const VerifyArgs& a, dial_dtype dt, void* ws, cudaStream_t st) {
