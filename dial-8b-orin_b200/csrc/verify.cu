@@ -28,6 +28,8 @@ constexpr int SEG = 1024;           // a warp's piece of a row
 constexpr int kStatWarps = 4;
 constexpr int kDrawThreads = 512;
 constexpr int kWarps = kDrawThreads / 32;
+constexpr int HOLD = 5;             // vectors that a thread of the draw keeps
+constexpr int kDrawSmem = HOLD * kDrawThreads * 24 + 64 * 32 * 8;
 
 struct __align__(16) SegStat {
   float m, s;                // maximum, sum of exp((x - m) / T)
@@ -188,25 +190,28 @@ __device__ const double kPow2[64] = {
     0x1.d5818dcfba487p+0, 0x1.da9e603db3285p+0, 0x1.dfc97337b9b5fp+0, 0x1.e502ee78b3ff6p+0,
     0x1.ea4afa2a490dap+0, 0x1.efa1bee615a27p+0, 0x1.f50765b6e4540p+0, 0x1.fa7c1819e90d8p+0};
 
-// exp((x - m) / T) up to a factor that all of a row share, x <= m finite, minus infinity or
-// NaN (both 0), to 2^-34: eight f64 operations.  Every lane has a copy of the table in its
-// own banks: entry j of lane l at table[32 j + l].
+// exp((x - m) / T) up to a factor that all of a row share, to 2^-34, in eight f64
+// operations.  Values 1000 octaves below the maximum, minus infinity and NaN give 2^-1000,
+// which no sum feels and kNone tells from a weight.  Every lane has a copy of the table in
+// its own banks: entry j of lane l at table[32 j + l].
+constexpr double kNone = 1e-290;
 struct Exp {
   const double* table;  // 2^(j / 64), this lane's
   double k, c;          // 64 log2(e) / T, minus m times that
-  __device__ __forceinline__ Exp(const double* t, float m, double k64) : table(t + (threadIdx.x & 31)), k(k64), c(-(double)m * k64) {}
+  float least;
+  __device__ __forceinline__ Exp(const double* t, float m, float temp, double k64)
+      : table(t + (threadIdx.x & 31)), k(k64), c(-(double)m * k64), least(fmaxf(m - 693.f * temp, -3e38f)) {}
   __device__ __forceinline__ double operator()(float x) const {
-    const double y = fma((double)x, k, c);
+    const double y = fma((double)fmaxf(x, least), k, c);
     const double t = y + 6755399441055744.0;            // 1.5 * 2^52: the integer in the low word
     const int n = __double2loint(t);
     const double r = y - (t - 6755399441055744.0);
-    double p = 2.1173137155464774e-07;                     // (ln2 / 64)^j / j!
+    double p = 2.1173137155464774e-07;                  // (ln2 / 64)^j / j!
     p = fma(p, r, 5.864904955056169e-05);
     p = fma(p, r, 0.010830424696249145);
     const double e = table[(n & 63) * 32];
     const double v = fma(e, p * r, e);
-    const double z = __hiloint2double(__double2hiint(v) + (n >> 6) * (1 << 20), __double2loint(v));
-    return y > -64000.0 ? z : 0.0;
+    return __hiloint2double(__double2hiint(v) + (n >> 6) * (1 << 20), __double2loint(v));
   }
 };
 
@@ -254,8 +259,8 @@ __device__ __forceinline__ double meet(double* sum, int rank, double mine, doubl
   double hit_before = 0.0, last_before = 0.0;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
-    if (v[i] > 0.0) last = lane * PER + i, last_before = cum;
-    if (hit == CL * kWarps && v[i] > 0.0 && cum + v[i] > at) hit = lane * PER + i, hit_before = cum;
+    if (v[i] > kNone) last = lane * PER + i, last_before = cum;
+    if (hit == CL * kWarps && v[i] > kNone && cum + v[i] > at) hit = lane * PER + i, hit_before = cum;
     cum += v[i];
   }
   const unsigned some = __ballot_sync(0xffffffffu, hit < CL * kWarps), any = __ballot_sync(0xffffffffu, last >= 0);
@@ -271,12 +276,15 @@ __device__ __forceinline__ double meet(double* sum, int rank, double mine, doubl
   return total;
 }
 
-template <typename T, int CL>
-__global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(kDrawThreads)
+template <typename T, int CL, int PER_SM>
+__global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(kDrawThreads, PER_SM)
     verify_draw_kernel(VerifyArgs a, const SegStat* __restrict__ stat, int nseg) {
-  constexpr int N = Vec<T>::N, HOLD = 5;  // vectors of a lane whose sums are kept
-  __shared__ __align__(16) double table[64 * 32], sum[2][CL * kWarps];  // a buffer is free again two meetings later
-  __shared__ double part[HOLD][kDrawThreads];
+  constexpr int N = Vec<T>::N;
+  __shared__ __align__(16) double sum[2][CL * kWarps];
+  extern __shared__ __align__(16) uint8_t draw_smem[];
+  uint4(*held)[kDrawThreads] = reinterpret_cast<uint4(*)[kDrawThreads]>(draw_smem);  // this thread's vectors
+  double(*part)[kDrawThreads] = reinterpret_cast<double(*)[kDrawThreads]>(draw_smem + HOLD * kDrawThreads * 16);  // their sums
+  double* table = reinterpret_cast<double*>(draw_smem + HOLD * kDrawThreads * 24);  // [64][32]
   __shared__ float row_m[kWarps], row_z[kWarps], row_x[kWarps];
   __shared__ int row_top[kWarps], row_ok[kWarps], row_draft[kWarps];
   pdl_trigger();
@@ -288,7 +296,7 @@ __global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(kDrawThreads)
   const Rows rw = rows_of(a, b, rank == 0 && threadIdx.x == 0);
   const int64_t V = a.vocab, total = a.rows * V;
   const T* x = static_cast<const T*>(a.logits);
-  const float temp = a.temperature[b], it = log2e_over(temp);
+  const float tb = a.temperature[b], temp = tb > 1e30f ? 1e30f : tb, it = log2e_over(temp);
   const float ut = a.sample_u[b];
   const bool greedy = !(temp > 0.f);
   const double k64 = greedy ? 0.0 : 92.332482616893656 / (double)temp;  // 64 log2(e) / T
@@ -299,7 +307,7 @@ __global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(kDrawThreads)
     return;  // the whole cluster: no rows
   }
 
-  // ---- acceptance, a warp per row, sixteen rows at a time
+  // ---- acceptance, a warp per row
   int64_t stop = rw.q1 - 1;
   float m = 0.f, Z = 0.f;
   int top = 0, draft = -1;
@@ -342,7 +350,7 @@ __global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(kDrawThreads)
     __syncthreads();
     const int n = (int)min((int64_t)kWarps, rw.q1 - r0);
     const unsigned good = __ballot_sync(0xffffffffu, lane < n && row_ok[lane & (kWarps - 1)]);
-    const int k = __ffs(~good) - 1;  // the accepted ones in front
+    const int k = good == 0xffffffffu ? 32 : __ffs(~good) - 1;  // the accepted ones in front
     if (rank == 0 && threadIdx.x < k) {
       a.out_ids[r0 + threadIdx.x] = row_draft[threadIdx.x];
       if (a.logprobs) a.logprobs[r0 + threadIdx.x] = log_p(row_x[threadIdx.x], row_m[threadIdx.x], row_z[threadIdx.x]);
@@ -374,7 +382,7 @@ __global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(kDrawThreads)
 
   // ---- the draw from row `stop`: run w of CL * kWarps, in whole vectors
   const bool inf = m == INFINITY;  // takes everything: weights 1 at the maximum
-  const Exp ex(table, inf ? 0.f : m, k64);
+  const Exp ex(table, inf ? 0.f : m, temp, k64);
   const int64_t lo = stop * V, hi = lo + V, v0 = lo / N, nv = (hi + N - 1) / N - v0;
   const int64_t per = (nv + CL * kWarps - 1) / (CL * kWarps);
   const int64_t a0 = v0 + min(nv, (int64_t)(rank * kWarps + warp) * per), a1 = min(v0 + nv, a0 + per);
@@ -382,6 +390,7 @@ __global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(kDrawThreads)
   // 0: all of p; 1: p without the draft; 2: max(p - q, 0), after a pass for Z in f64
   const int kind = !rejected ? 0 : (a.probs ? 2 : 1);
   int mode = kind == 2 ? 0 : kind;
+  const int64_t dv = mode == 1 && draft >= 0 && draft < V ? (lo + draft) / N : -1;  // the draft's vector
   auto weights = [&](uint4 u, int64_t v, double (&w)[N]) {
     float f[N];
     Vec<T>::template values<true>(u, v, lo, hi, f);
@@ -389,14 +398,14 @@ __global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(kDrawThreads)
 #pragma unroll
       for (int i = 0; i < N; ++i) f[i] = f[i] == m ? 0.f : -INFINITY;
     }
-#pragma unroll
-    for (int i = 0; i < N; ++i) w[i] = ex(f[i]);
-    if (mode == 1) {
-      const int64_t at = lo + draft - v * N;
+    if (v == dv && mode == 1) {
 #pragma unroll
       for (int i = 0; i < N; ++i)
-        if (i == at) w[i] = 0.0;
-    } else if (mode == 2) {  // max(p - q, 0) Z = max(e - q Z, 0)
+        if (v * N + i == lo + draft) f[i] = -INFINITY;
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) w[i] = ex(f[i]);
+    if (mode == 2) {  // max(p - q, 0) Z = max(e - q Z, 0)
       float q[N];
       if ((v + 1) * N <= total) {
 #pragma unroll
@@ -409,15 +418,18 @@ __global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(kDrawThreads)
         for (int i = 0; i < N; ++i) q[i] = v * N + i < total ? a.probs[v * N + i] : 0.f;
       }
 #pragma unroll
-      for (int i = 0; i < N; ++i)  // (outside the row w is 0 and stays it)
-        w[i] = fmax(fma(-(double)q[i], z64, w[i]), 0.0);
+      for (int i = 0; i < N; ++i) {  // (outside the row w is nothing and stays it)
+        const double d = fma(-(double)q[i], z64, w[i]);
+        w[i] = __double2hiint(d) < 0 ? 0.0 : d;
+      }
     }
   };
   auto weight1 = [&](int64_t e) {  // of one element of the row
     float f = Act<T>::to_f32(x[e]);
     if (inf) f = f == m ? 0.f : -INFINITY;
+    if (mode == 1 && e - lo == draft) f = -INFINITY;
     const double w = ex(f);
-    return mode == 1 ? (e - lo == draft ? 0.0 : w) : mode == 2 ? fmax(fma(-(double)a.probs[e], z64, w), 0.0) : w;
+    return mode == 2 ? fmax(fma(-(double)a.probs[e], z64, w), 0.0) : w;
   };
   if (kind == 2)  // the draft's weights of this run, wanted after the pass for Z
     for (int64_t e = a0 * N + 32 * lane; e < min(a1 * N, total); e += 32 * 32)
@@ -426,6 +438,7 @@ __global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(kDrawThreads)
   cluster_wait();
   const double u = (double)ut;
   const bool single = per <= 32 * HOLD;  // all sums of the run are kept
+  bool loaded = false;
   int run = -1, buf = 0, token = -1;
   double before = 0.0, all = 0.0, at = 0.0;
   // passes over the run: for Z, for the weights, and for the place of `at`.  The loops stay
@@ -437,16 +450,27 @@ __global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(kDrawThreads)
 #pragma unroll 1
     for (int64_t c0 = a0; c0 < a1 && !found; c0 += 32 * HOLD) {
       if (!locate || !single) {
-        uint4 next = c0 + lane < a1 ? Vec<T>::load(x, c0 + lane, total) : make_uint4(0, 0, 0, 0);
+        if (!single || !loaded) {  // all in flight at once; each thread reads back its own
+#pragma unroll
+          for (int k = 0; k < HOLD; ++k) {
+            const int64_t v = c0 + 32 * k + lane;
+            if (v < a1 && (v + 1) * N <= total)
+              asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(&held[k][threadIdx.x])),
+                           "l"(reinterpret_cast<const uint4*>(x) + v)
+                           : "memory");
+            else if (v < a1)
+              held[k][threadIdx.x] = Vec<T>::load(x, v, total);
+          }
+          asm volatile("cp.async.wait_all;" ::: "memory");
+          loaded = true;
+        }
 #pragma unroll 1
         for (int k = 0; k < HOLD; ++k) {
           const int64_t v = c0 + 32 * k + lane;
-          const uint4 now = next;
-          if (v + 32 < a1) next = Vec<T>::load(x, v + 32, total);
           double s = 0.0;
           if (v < a1) {
             double w[N];
-            weights(now, v, w);
+            weights(held[k][threadIdx.x], v, w);
 #pragma unroll
             for (int i = 0; i < N; i += 2) s += w[i] + w[i + 1];
           }
@@ -467,8 +491,8 @@ __global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(kDrawThreads)
           const double y = __shfl_up_sync(0xffffffffu, pre, o);
           if (lane >= o) pre += y;
         }
-        const unsigned some = __ballot_sync(0xffffffffu, s > 0.0 && cum + pre > at);
-        const unsigned any = __ballot_sync(0xffffffffu, s > 0.0);
+        const unsigned some = __ballot_sync(0xffffffffu, s > kNone && cum + pre > at);
+        const unsigned any = __ballot_sync(0xffffffffu, s > kNone);
         if (any) {
           const int l = some ? __ffs(some) - 1 : 31 - __clz(any);
           vec = c0 + 32 * k + l;
@@ -486,8 +510,8 @@ __global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(kDrawThreads)
           const double y = __shfl_up_sync(0xffffffffu, pre, o);
           if (lane >= o) pre += y;
         }
-        const unsigned some = __ballot_sync(0xffffffffu, w > 0.0 && start + pre > at);
-        const unsigned any = __ballot_sync(0xffffffffu, w > 0.0);
+        const unsigned some = __ballot_sync(0xffffffffu, w > kNone && start + pre > at);
+        const unsigned any = __ballot_sync(0xffffffffu, w > kNone);
         token = (int)(vec * N + (some ? __ffs(some) - 1 : 31 - __clz(any)) - lo);
       }
     }
@@ -500,7 +524,7 @@ __global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(kDrawThreads)
     if (kind == 2 && z64 == 0.0) {
       z64 = all;
       mode = 2;
-    } else if (mode && !(all > 0.0)) {
+    } else if (mode && !(all > kNone)) {
       mode = 0;  // nothing left of it: from p
     } else {
       if (r != rank * kWarps + warp) break;
@@ -525,6 +549,14 @@ size_t verify_workspace_bytes(int64_t rows, int64_t vocab) {
   return (size_t)(rows * segments(vocab)) * sizeof(SegStat);
 }
 
+template <typename T, int CL, int PER_SM>
+static dial_status launch_draw(const VerifyArgs& a, const SegStat* stat, int nseg, cudaStream_t st) {
+  const cudaError_t e = ensure_smem<verify_draw_kernel<T, CL, PER_SM>>(kDrawSmem);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(verify_draw_kernel)");
+  return launch_pdl("verify_draw_kernel", verify_draw_kernel<T, CL, PER_SM>, dim3((unsigned)(a.n_seqs * CL)), dim3(kDrawThreads),
+                    kDrawSmem, st, a, stat, nseg);
+}
+
 template <typename T>
 static dial_status verify_t(const VerifyArgs& a, void* ws, cudaStream_t st) {
   const int64_t nseg = segments(a.vocab), blocks = (a.rows * nseg + kStatWarps - 1) / kStatWarps;
@@ -533,13 +565,14 @@ static dial_status verify_t(const VerifyArgs& a, void* ws, cudaStream_t st) {
   const dial_status s = launch_pdl("verify_stats_kernel", verify_stats_kernel<T>, dim3((unsigned)blocks),
                                    dim3(kStatWarps * 32), 0, st, a, stat, (int)nseg);
   if (s != DIAL_OK) return s;
-  // CTAs per sequence: as many as leave every CTA an SM of its own (eight at most: the
-  // portable cluster), two from 74 sequences on
-  const int sms = sm_count();
-  const int cl = a.n_seqs * 8 <= sms ? 8 : (a.n_seqs * 4 <= sms ? 4 : 2);
-  auto k = cl == 8 ? verify_draw_kernel<T, 8> : (cl == 4 ? verify_draw_kernel<T, 4> : verify_draw_kernel<T, 2>);
-  return launch_pdl("verify_draw_kernel", k, dim3((unsigned)(a.n_seqs * cl)), dim3(kDrawThreads), 0, st, a, stat,
-                    (int)nseg);
+  // CTAs per sequence: eight (the portable cluster) while they have an SM each or share it
+  // with one other (64 registers then: 12.7 -> 14.0 us for one sequence, but 49 -> 39 us for
+  // 32 against four CTAs each), then fewer
+  const int64_t ctas = 8 * (int64_t)a.n_seqs, sms = sm_count();
+  return ctas <= sms       ? launch_draw<T, 8, 1>(a, stat, (int)nseg, st)
+         : ctas <= 2 * sms ? launch_draw<T, 8, 2>(a, stat, (int)nseg, st)
+         : ctas <= 4 * sms ? launch_draw<T, 4, 2>(a, stat, (int)nseg, st)
+                           : launch_draw<T, 2, 2>(a, stat, (int)nseg, st);
 }
 
 dial_status launch_verify(const VerifyArgs& a, dial_dtype dt, void* ws, cudaStream_t st) {
