@@ -46,28 +46,44 @@ class _RopeAxes(ctypes.Structure):
     _fields_ = [("n_axes", ctypes.c_int32), ("section", ctypes.c_int32 * 4), ("interleaved", ctypes.c_int32)]
 
 
-def _tensor(t, name: str, dtype=None, shape: Optional[tuple] = None, device=None):
+def _tensor(t, name: str, dtype, shape: tuple, index: int):
+    """t: a contiguous `dtype` tensor of `shape` on CUDA device `index`."""
+    if t.dtype is dtype and t.shape == shape and t.get_device() == index and t.is_contiguous():
+        return
     if not t.is_cuda:
         raise RuntimeError(f"{name}: dial_cuda ops take CUDA tensors; there is no CPU path")
     if not t.is_contiguous():
         raise RuntimeError(f"{name}: dial_cuda ops take contiguous tensors")
-    if dtype is not None and t.dtype != dtype:
+    if t.dtype is not dtype:
         raise TypeError(f"{name}: expected {dtype}, got {t.dtype}")
-    if shape is not None and tuple(t.shape) != shape:
+    if t.shape != shape:
         raise ValueError(f"{name}: expected shape {shape}, got {tuple(t.shape)}")
-    if device is not None and t.device != device:
-        raise RuntimeError(f"{name}: on {t.device}, the others on {device}")
-    return t
+    raise RuntimeError(f"{name}: on {t.device}, the others on cuda:{index}")
 
 
-def _call(name: str, device, *args):
-    """A library call on the current stream of `device` (made current for the call)."""
+_fns = {}
+
+
+def _call(name: str, index: int, *args):
+    """A library call on the current stream of CUDA device `index` (made current for the call)."""
     torch = _torch()
-    if device.index == torch.cuda.current_device():
-        check(getattr(lib(), name)(*args, torch.cuda.current_stream().cuda_stream), name)
+    fn = _fns.get(name)
+    if fn is None:
+        fn = _fns[name] = getattr(lib(), name)
+    if index == torch.cuda.current_device():
+        status = fn(*args, _raw_stream(index))
     else:
-        with torch.cuda.device(device):
-            check(getattr(lib(), name)(*args, torch.cuda.current_stream().cuda_stream), name)
+        with torch.cuda.device(index):
+            status = fn(*args, _raw_stream(index))
+    if status:
+        check(status, name)
+
+
+def _raw_stream(index: int) -> int:
+    """The current stream's cudaStream_t; without the Stream object that costs 3 us a call."""
+    torch = _torch()
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return raw(index) if raw is not None else torch.cuda.current_stream(index).cuda_stream
 
 
 class PagedBatch:
@@ -81,17 +97,17 @@ class PagedBatch:
 
     def __init__(self, block_table, kv_len, q_start, max_q: Optional[int] = None, max_kv: Optional[int] = None):
         torch = _torch()
-        dev = block_table.device
-        _tensor(block_table, "block_table", torch.int32)
         if block_table.dim() != 2 or 0 in block_table.shape:
             raise ValueError(f"block_table must be [n_seqs, max_pages], got {tuple(block_table.shape)}")
         n, pages = block_table.shape
-        _tensor(kv_len, "kv_len", torch.int32, (n,), dev)
-        _tensor(q_start, "q_start", torch.int32, (n + 1,), dev)
+        index = max(block_table.get_device(), 0)
+        _tensor(block_table, "block_table", torch.int32, (n, pages), index)
+        _tensor(kv_len, "kv_len", torch.int32, (n,), index)
+        _tensor(q_start, "q_start", torch.int32, (n + 1,), index)
         for name, v in (("max_q", max_q), ("max_kv", max_kv)):
             if v is not None and v <= 0:
                 raise ValueError(f"{name} must be positive (got {v})")
-        self.block_table, self.kv_len, self.q_start, self.device = block_table, kv_len, q_start, dev
+        self.block_table, self.kv_len, self.q_start, self._index = block_table, kv_len, q_start, index
         self.n_seqs, self.max_pages, self.max_q, self.max_kv = n, pages, max_q, max_kv
         self._c = {}
 
@@ -139,14 +155,16 @@ class PagedKVCache:
         self.quantized = k.dtype == torch.int8
         if self.quantized != (ks is not None) or self.quantized != (vs is not None):
             raise ValueError("int8 pages, and only they, have k_scale and v_scale")
-        _tensor(k, "k_pages")
-        _tensor(v, "v_pages", k.dtype, tuple(k.shape), k.device)
+        index = max(k.get_device(), 0)
+        _tensor(k, "k_pages", k.dtype, k.shape, index)
+        _tensor(v, "v_pages", k.dtype, k.shape, index)
         for name, s in (("k_scale", ks), ("v_scale", vs)):
             if s is not None:
-                _tensor(s, name, torch.float32, tuple(k.shape[:3]), k.device)
+                _tensor(s, name, torch.float32, k.shape[:3], index)
         self.k_pages, self.v_pages, self.k_scale, self.v_scale = k, v, ks, vs
         self.n_pages, self.n_kv_heads, self.page_size, _ = k.shape
-        self.device = k.device
+        self.device, self._index = k.device, index
+        self._codes = {torch.float16: 1, torch.bfloat16: 2} if self.quantized else {k.dtype: dtype_code(k.dtype)}
         self._c = _byref(_PagedKv(k.data_ptr(), v.data_ptr(), ks.data_ptr() if ks is not None else None,
                                   vs.data_ptr() if vs is not None else None,
                                   KV_INT8 if self.quantized else dtype_code(k.dtype), self.n_kv_heads, 128,
@@ -157,17 +175,17 @@ class PagedKVCache:
         b = 2 * self.k_pages.numel() * self.k_pages.element_size()
         return b + (2 * self.k_scale.numel() * 4 if self.quantized else 0)
 
-    def _act(self, t, name: str):
-        torch = _torch()
-        _tensor(t, name, None if self.quantized else self.k_pages.dtype, None, self.device)
-        if t.dtype not in (torch.float16, torch.bfloat16):
-            raise TypeError(f"{name}: expected f16 or bf16, got {t.dtype}")
-        return dtype_code(t.dtype)
+    def _act(self, t, name: str) -> int:
+        """The code of an activation tensor's type."""
+        code = self._codes.get(t.dtype)
+        if code is None:
+            raise TypeError(f"{name}: expected {' or '.join(map(str, self._codes))}, got {t.dtype}")
+        return code
 
     def _batch(self, batch: PagedBatch):
-        if batch.device != self.device:
-            raise RuntimeError(f"batch: on {batch.device}, the cache on {self.device}")
-        return batch._struct(self.page_size)
+        if batch._index != self._index:
+            raise RuntimeError(f"batch: on cuda:{batch._index}, the cache on cuda:{self._index}")
+        return batch._c.get(self.page_size) or batch._struct(self.page_size)
 
     def append(self, qkv, batch: PagedBatch, cos, sin, positions, q_norm=None, k_norm=None, eps: float = 1e-6,
                sections: Sequence[int] = (64,), interleaved: bool = True, out=None):
@@ -178,51 +196,45 @@ class PagedKVCache:
         one axis per entry of `sections` (pairs of each axis, summing to 64; interleaved as
         Qwen3-VL, or consecutive).  q_norm, k_norm: [128] weights, or neither."""
         torch = _torch()
-        dt = self._act(qkv, "qkv")
-        T, dev = qkv.shape[0], self.device
-        hq = qkv.shape[1] // 128 - 2 * self.n_kv_heads if qkv.dim() == 2 else 0
+        dt, index, n = self._act(qkv, "qkv"), self._index, len(sections)
+        T, hq = qkv.shape[0], qkv.shape[1] // 128 - 2 * self.n_kv_heads if qkv.dim() == 2 else 0
         if hq <= 0 or qkv.shape[1] % 128:
             raise ValueError(f"qkv must be [T, (Hq + 2 * {self.n_kv_heads}) * 128], got {tuple(qkv.shape)}")
-        n = len(sections)
-        if not 1 <= n <= 4:
-            raise ValueError(f"1 to 4 position axes, got {n}")
-        if positions.numel() != n * T or positions.shape[-1] != T:
-            raise ValueError(f"positions must be [{n}, {T}], got {tuple(positions.shape)}")
-        _tensor(positions, "positions", torch.int32, None, dev)
-        _tensor(cos, "cos", torch.float32, (cos.shape[0], 64), dev)
-        _tensor(sin, "sin", torch.float32, tuple(cos.shape), dev)
+        _tensor(qkv, "qkv", qkv.dtype, (T, (hq + 2 * self.n_kv_heads) * 128), index)
+        axes = _axes(tuple(sections), bool(interleaved))
+        _tensor(positions, "positions", torch.int32, (T,) if n == 1 and positions.dim() == 1 else (n, T), index)
+        rows = cos.shape[0]
+        _tensor(cos, "cos", torch.float32, (rows, 64), index)
+        _tensor(sin, "sin", torch.float32, (rows, 64), index)
         if (q_norm is None) != (k_norm is None):
             raise ValueError("q_norm and k_norm go together")
-        for name, w in (("q_norm", q_norm), ("k_norm", k_norm)):
-            if w is not None:
-                _tensor(w, name, qkv.dtype, (128,), dev)
+        if q_norm is not None:
+            _tensor(q_norm, "q_norm", qkv.dtype, (128,), index)
+            _tensor(k_norm, "k_norm", qkv.dtype, (128,), index)
         if out is None:
-            out = torch.empty((T, hq, 128), dtype=qkv.dtype, device=dev)
+            out = torch.empty((T, hq, 128), dtype=qkv.dtype, device=self.device)
         else:
-            _tensor(out, "out", qkv.dtype, (T, hq, 128), dev)
-        if T == 0:
-            return out
-        axes = _RopeAxes(n, (ctypes.c_int32 * 4)(*sections), int(interleaved))
-        _call("dial_paged_kv_append", dev, qkv.data_ptr(), q_norm.data_ptr() if q_norm is not None else None,
-              k_norm.data_ptr() if k_norm is not None else None, cos.data_ptr(), sin.data_ptr(), cos.shape[0],
-              positions.data_ptr(), _byref(axes), self._c, self._batch(batch), out.data_ptr(), dt, T, hq, eps)
+            _tensor(out, "out", qkv.dtype, (T, hq, 128), index)
+        if T:
+            _call("dial_paged_kv_append", index, qkv.data_ptr(), q_norm.data_ptr() if q_norm is not None else None,
+                  k_norm.data_ptr() if k_norm is not None else None, cos.data_ptr(), sin.data_ptr(), rows,
+                  positions.data_ptr(), axes, self._c, self._batch(batch), out.data_ptr(), dt, T, hq, eps)
         return out
 
     def attention(self, q, batch: PagedBatch, scale: Optional[float] = None, out=None):
         """Attention of the batch's tokens, q [T, Hq, 128] -> [T, Hq, 128]: each attends its
         sequence's rows up to its own.  scale: 1/sqrt(128) by default."""
-        torch = _torch()
-        dt = self._act(q, "q")
-        if q.dim() != 3 or q.shape[2] != 128:
-            raise ValueError(f"q must be [T, Hq, 128], got {tuple(q.shape)}")
+        dt, shape, index = self._act(q, "q"), q.shape, self._index
+        if len(shape) != 3 or shape[2] != 128:
+            raise ValueError(f"q must be [T, Hq, 128], got {tuple(shape)}")
+        _tensor(q, "q", q.dtype, shape, index)
         if out is None:
-            out = torch.empty_like(q)
+            out = _torch().empty_like(q)
         else:
-            _tensor(out, "out", q.dtype, tuple(q.shape), self.device)
-        if q.shape[0] == 0:
-            return out
-        _call("dial_paged_attention", self.device, q.data_ptr(), self._c, self._batch(batch), out.data_ptr(), dt,
-              q.shape[0], q.shape[1], 0.08838834764831845 if scale is None else scale)
+            _tensor(out, "out", q.dtype, shape, index)
+        if shape[0]:
+            _call("dial_paged_attention", index, q.data_ptr(), self._c, self._batch(batch), out.data_ptr(), dt, shape[0],
+                  shape[1], 0.08838834764831845 if scale is None else scale)
         return out
 
     def read(self, batch: PagedBatch, tokens: Optional[int] = None, dtype=None, out=None) -> Tuple:
@@ -235,14 +247,29 @@ class PagedKVCache:
             dtype = dtype or (torch.float16 if self.quantized else self.k_pages.dtype)
             out = tuple(torch.empty((tokens, self.n_kv_heads, 128), dtype=dtype, device=self.device) for _ in range(2))
         k, v = out
-        dt = self._act(k, "out[0]")
-        if k.dim() != 3 or tuple(k.shape[1:]) != (self.n_kv_heads, 128):
-            raise ValueError(f"out must be [T, {self.n_kv_heads}, 128], got {tuple(k.shape)}")
-        _tensor(v, "out[1]", k.dtype, tuple(k.shape), self.device)
-        if k.shape[0]:
-            _call("dial_paged_kv_read", self.device, self._c, self._batch(batch), k.data_ptr(), v.data_ptr(), dt,
-                  k.shape[0])
+        dt, shape, index = self._act(k, "out[0]"), k.shape, self._index
+        if len(shape) != 3 or shape[1:] != (self.n_kv_heads, 128):
+            raise ValueError(f"out must be [T, {self.n_kv_heads}, 128], got {tuple(shape)}")
+        _tensor(k, "out[0]", k.dtype, shape, index)
+        _tensor(v, "out[1]", k.dtype, shape, index)
+        if shape[0]:
+            _call("dial_paged_kv_read", index, self._c, self._batch(batch), k.data_ptr(), v.data_ptr(), dt, shape[0])
         return k, v
+
+
+_AXES = {}
+
+
+def _axes(sections: tuple, interleaved: bool):
+    """The dial_rope_axes of these sections, made once."""
+    a = _AXES.get((sections, interleaved))
+    if a is None:
+        if not 1 <= len(sections) <= 4:
+            raise ValueError(f"1 to 4 position axes, got {len(sections)}")
+        a = _byref(_RopeAxes(len(sections), (ctypes.c_int32 * 4)(*sections), int(interleaved)))
+        if len(_AXES) < 64:
+            _AXES[sections, interleaved] = a
+    return a
 
 
 def rope_tables(rows: int, theta: float, device=None):
@@ -251,7 +278,7 @@ def rope_tables(rows: int, theta: float, device=None):
     device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
     cos = torch.empty((rows, 64), dtype=torch.float32, device=device)
     sin = torch.empty_like(cos)
-    _call("dial_rope_tables", cos.device, cos.data_ptr(), sin.data_ptr(), dtype_code(torch.float32), rows, 128, theta)
+    _call("dial_rope_tables", cos.get_device(), cos.data_ptr(), sin.data_ptr(), dtype_code(torch.float32), rows, 128, theta)
     return cos, sin
 
 
@@ -268,28 +295,30 @@ def verify_drafts(logits, ids, q_start, temperature, accept_u, sample_u, draft_p
     [R]): the accepted drafts and the drawn token of each sequence, -1 behind them.  Rows
     from q_start[n_seqs] on belong to no sequence and are not written."""
     torch = _torch()
-    dev = logits.device
-    _tensor(logits, "logits")
+    index = max(logits.get_device(), 0)
     if logits.dim() != 2 or 0 in logits.shape:
         raise ValueError(f"logits must be [R, V], got {tuple(logits.shape)}")
     R, V = logits.shape
     n = q_start.numel() - 1
     if n < 1:
         raise ValueError("q_start must hold n_seqs + 1 values")
-    _tensor(ids, "ids", torch.int32, (R,), dev)
-    _tensor(q_start, "q_start", torch.int32, (n + 1,), dev)
-    _tensor(temperature, "temperature", torch.float32, (n,), dev)
-    _tensor(accept_u, "accept_u", torch.float32, (R,), dev)
-    _tensor(sample_u, "sample_u", torch.float32, (n,), dev)
+    f32, i32 = torch.float32, torch.int32
+    _tensor(logits, "logits", logits.dtype, (R, V), index)
+    _tensor(ids, "ids", i32, (R,), index)
+    _tensor(q_start, "q_start", i32, (n + 1,), index)
+    _tensor(temperature, "temperature", f32, (n,), index)
+    _tensor(accept_u, "accept_u", f32, (R,), index)
+    _tensor(sample_u, "sample_u", f32, (n,), index)
     if draft_probs is not None:
-        _tensor(draft_probs, "draft_probs", torch.float32, (R, V), dev)
-    out = torch.empty(R, dtype=torch.int32, device=dev)
-    count = torch.empty(n, dtype=torch.int32, device=dev)
-    logp = torch.empty(R, dtype=torch.float32, device=dev)
+        _tensor(draft_probs, "draft_probs", f32, (R, V), index)
+    # one allocation: tokens, counts, log-probabilities, workspace
     need = lib().dial_verify_drafts_workspace_bytes(R, V)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev)
-    _call("dial_verify_drafts", dev, logits.data_ptr(), dtype_code(logits.dtype), ids.data_ptr(),
+    at = (2 * R + n + 3) // 4 * 4
+    buf = torch.empty(at + need // 4, dtype=i32, device=logits.device)
+    out, count, logp, _ = buf.split((R, n, R, buf.numel() - 2 * R - n))
+    p = buf.data_ptr()
+    _call("dial_verify_drafts", index, logits.data_ptr(), dtype_code(logits.dtype), ids.data_ptr(),
           draft_probs.data_ptr() if draft_probs is not None else None, q_start.data_ptr(), n,
-          temperature.data_ptr(), accept_u.data_ptr(), sample_u.data_ptr(), out.data_ptr(), count.data_ptr(),
-          logp.data_ptr(), R, V, max_q or R, ws.data_ptr(), need)
-    return out, count, logp
+          temperature.data_ptr(), accept_u.data_ptr(), sample_u.data_ptr(), p, p + 4 * R, p + 4 * (R + n),
+          R, V, max_q or R, p + 4 * at, need)
+    return out, count, logp.view(f32)
