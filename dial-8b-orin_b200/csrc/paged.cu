@@ -10,19 +10,38 @@ namespace {
 
 constexpr int D = 128;
 
+// Four values as two pairs.
 template <typename T>
-__device__ __forceinline__ void unpack4(uint2 u, float (&v)[4]) {
-  const T* h = reinterpret_cast<const T*>(&u);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = Act<T>::to_f32(h[i]);
+__device__ __forceinline__ void unpack4(uint2 u, float2 (&v)[2]);
+template <>
+__device__ __forceinline__ void unpack4<__half>(uint2 u, float2 (&v)[2]) {
+  v[0] = __half22float2(*reinterpret_cast<const __half2*>(&u.x));
+  v[1] = __half22float2(*reinterpret_cast<const __half2*>(&u.y));
+}
+template <>
+__device__ __forceinline__ void unpack4<__nv_bfloat16>(uint2 u, float2 (&v)[2]) {
+  v[0] = make_float2(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xFFFF0000u));
+  v[1] = make_float2(__uint_as_float(u.y << 16), __uint_as_float(u.y & 0xFFFF0000u));
 }
 template <typename T>
-__device__ __forceinline__ uint2 pack4(const float (&v)[4]) {
-  uint2 u;
-  T* h = reinterpret_cast<T*>(&u);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) h[i] = Act<T>::from_f32(v[i]);
-  return u;
+__device__ __forceinline__ uint2 pack4(const float2 (&v)[2]);
+template <>
+__device__ __forceinline__ uint2 pack4<__half>(const float2 (&v)[2]) {
+  const __half2 a = __float22half2_rn(v[0]), b = __float22half2_rn(v[1]);
+  return make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+}
+template <>
+__device__ __forceinline__ uint2 pack4<__nv_bfloat16>(const float2 (&v)[2]) {
+  const __nv_bfloat162 a = __float22bfloat162_rn(v[0]), b = __float22bfloat162_rn(v[1]);
+  return make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n .reg .b64 a, b, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n mul.rn.f32x2 d, a, b;\n"
+      " mov.b64 {%0, %1}, d;\n}\n"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
 }
 
 // Row scale and reciprocal of the int8 rows: absmax / 127, 1 for rows without
@@ -40,31 +59,32 @@ __device__ __forceinline__ uint32_t code(float x, float inv) {
 
 // ------------------------------------------------------------------ append
 // A half-warp per head: lane j of 16 holds elements 4j .. 4j+3 and 64+4j .. 64+4j+3, so
-// the pairs (i, i + 64) stay in the lane.  A CTA is one token (or a part of its heads): the
-// page row and the token's cosines are looked up once and every half-warp walks heads, the
-// next one's values on their way while it works on one.  Bound by the bytes of qkv, q and
-// the cache rows.
+// the pairs (i, i + 64) stay in the lane.  `wpt` warps share a token: each looks up the page
+// row and the token's cosines, then walks heads, the next one's values on their way while
+// it works on one.  Few tokens: a head each; many: as few warps a token as fill the SMs, as
+// the look-ups cost about what a head does.  Bound by the bytes of qkv, q and the cache rows.
 // The mean square is summed in f64 (its squares are exact there) and 1/sqrt refined by one
 // Newton step in f64, so that the f32 factor -- and with it every int8 code -- does not
 // depend on the order of a sum; each later product is rounded to f32 on its own for the
 // same reason.
 template <typename T, bool Q8>
 __global__ void __launch_bounds__(256)
-    paged_append_kernel(const T* __restrict__ qkv, RopeArgs r, PagedView p, T* __restrict__ q_out, int hq) {
+    paged_append_kernel(const T* __restrict__ qkv, RopeArgs r, PagedView p, T* __restrict__ q_out, int hq, int wpt) {
   pdl_begin();
-  const int64_t t = blockIdx.x;
-  const int heads = hq + 2 * p.hkv, step = gridDim.y * 16;
+  const int64_t w = blockIdx.x * (int64_t)(blockDim.x >> 5) + (threadIdx.x >> 5), t = w / wpt;
+  if (blockIdx.x == 0)
+    for (int b = threadIdx.x; b < p.n_seqs; b += blockDim.x) chunk_of(p, b, true);
+  if (t >= p.tokens) return;
+  const int heads = hq + 2 * p.hkv, step = 2 * wpt;
   const int j = threadIdx.x & 15;
   const unsigned half = 0xFFFFu << (threadIdx.x & 16);
-  int h = blockIdx.y * 16 + (threadIdx.x >> 4);
-  const T* tok = qkv + t * heads * D;
+  int h = (int)(w - t * wpt) * 2 + ((threadIdx.x >> 4) & 1);
+  const T* tok = qkv + (t * heads + h) * D;  // of head h
   uint2 na = make_uint2(0, 0), nz = na;
   if (h < heads) {
-    na = __ldg(reinterpret_cast<const uint2*>(tok + h * D) + j);
-    nz = __ldg(reinterpret_cast<const uint2*>(tok + h * D + 64) + j);
+    na = __ldg(reinterpret_cast<const uint2*>(tok) + j);
+    nz = __ldg(reinterpret_cast<const uint2*>(tok + 64) + j);
   }
-  if (t == 0 && blockIdx.y == 0)
-    for (int b = threadIdx.x; b < p.n_seqs; b += blockDim.x) chunk_of(p, b, true);
   const int b = seq_of_token(p, t);
   if (b >= p.n_seqs) return;  // behind the last sequence
   const Chunk c = chunk_of(p, b, false);
@@ -104,55 +124,67 @@ __global__ void __launch_bounds__(256)
   if (at >= 0) {
     const int page = __ldg(p.table + (int64_t)b * p.max_pages + (at >> p.log2_page));
     if (page < 0 || page >= p.n_pages) {
-      if (threadIdx.x == 0) flag_invalid(p.err);
+      flag_invalid(p.err);
     } else {
       row0 = (((int64_t)page * p.hkv) << p.log2_page) + (at & ((1 << p.log2_page) - 1));
     }
   }
-  for (; h < heads; h += step) {
-    float a[4], z[4];
+  const float2 cp[2] = {{cs[0], cs[1]}, {cs[2], cs[3]}}, sp[2] = {{sn[0], sn[1]}, {sn[2], sn[3]}};
+  float2 wa[2] = {}, wz[2] = {};  // norm weights of the heads at hand: q's, then k's
+  int kind = 0;
+  T* qdst = q_out + t * hq * D + h * D + 4 * j;
+  for (; h < heads; h += step, tok += step * D, qdst += step * D) {
+    float2 a[2], z[2];
     unpack4<T>(na, a);
     unpack4<T>(nz, z);
     if (h + step < heads) {
-      na = __ldg(reinterpret_cast<const uint2*>(tok + (h + step) * D) + j);
-      nz = __ldg(reinterpret_cast<const uint2*>(tok + (h + step) * D + 64) + j);
+      na = __ldg(reinterpret_cast<const uint2*>(tok + step * D) + j);
+      nz = __ldg(reinterpret_cast<const uint2*>(tok + step * D + 64) + j);
     }
     if (h < hq + p.hkv) {
-      const T* w = static_cast<const T*>(h < hq ? r.qn : r.kn);
-      if (w) {
-        float wa[4], wz[4];
-        unpack4<T>(__ldg(reinterpret_cast<const uint2*>(w) + j), wa);
-        unpack4<T>(__ldg(reinterpret_cast<const uint2*>(w + 64) + j), wz);
-        double ss = 0.0;
+      if (r.qn) {
+        const int now = h < hq ? 1 : 2;
+        if (now != kind) {
+          const T* w = static_cast<const T*>(h < hq ? r.qn : r.kn);
+          unpack4<T>(__ldg(reinterpret_cast<const uint2*>(w) + j), wa);
+          unpack4<T>(__ldg(reinterpret_cast<const uint2*>(w + 64) + j), wz);
+          kind = now;
+        }
+        const double d[8] = {a[0].x, a[0].y, a[1].x, a[1].y, z[0].x, z[0].y, z[1].x, z[1].y};
+        double ss = d[0] * d[0], s2 = d[4] * d[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) ss += (double)a[i] * a[i] + (double)z[i] * z[i];
+        for (int i = 1; i < 4; ++i) ss = fma(d[i], d[i], ss), s2 = fma(d[4 + i], d[4 + i], s2);
+        ss += s2;
 #pragma unroll
         for (int o = 8; o > 0; o >>= 1) ss += __shfl_xor_sync(half, ss, o);
-        const double m = ss / D + (double)r.eps;
+        const double m = fma(ss, 1.0 / D, (double)r.eps);
+        const float mf = (float)m;
         double y;
-        if (m > 1e-30 && m < 1e30) {
-          y = (double)rsqrtf((float)m);
-          y = y * (1.5 - 0.5 * m * y * y);
+        if (mf > 1e-30f && mf < 1e30f) {
+          y = (double)rsqrtf(mf);
+          y = y * fma(-0.5 * m * y, y, 1.5);
         } else {
           y = 1.0 / sqrt(m);
         }
         const float inv = (float)y;
+        const float2 iv = make_float2(inv, inv);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          a[i] = __fmul_rn(__fmul_rn(a[i], inv), wa[i]);
-          z[i] = __fmul_rn(__fmul_rn(z[i], inv), wz[i]);
+        for (int i = 0; i < 2; ++i) {
+          a[i] = mul2(mul2(a[i], iv), wa[i]);
+          z[i] = mul2(mul2(z[i], iv), wz[i]);
         }
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float x = a[i], y = z[i];
-        a[i] = __fsub_rn(__fmul_rn(x, cs[i]), __fmul_rn(y, sn[i]));
-        z[i] = __fadd_rn(__fmul_rn(x, sn[i]), __fmul_rn(y, cs[i]));
+      for (int i = 0; i < 2; ++i) {
+        const float2 x = a[i], y = z[i];
+        a[i].x = __fsub_rn(__fmul_rn(x.x, cp[i].x), __fmul_rn(y.x, sp[i].x));
+        a[i].y = __fsub_rn(__fmul_rn(x.y, cp[i].y), __fmul_rn(y.y, sp[i].y));
+        z[i].x = __fadd_rn(__fmul_rn(x.x, sp[i].x), __fmul_rn(y.x, cp[i].x));
+        z[i].y = __fadd_rn(__fmul_rn(x.y, sp[i].y), __fmul_rn(y.y, cp[i].y));
       }
       if (h < hq) {
-        T* dst = q_out + (t * hq + h) * D;
-        reinterpret_cast<uint2*>(dst)[j] = pack4<T>(a);
-        reinterpret_cast<uint2*>(dst + 64)[j] = pack4<T>(z);
+        *reinterpret_cast<uint2*>(qdst) = pack4<T>(a);
+        *reinterpret_cast<uint2*>(qdst + 64) = pack4<T>(z);
         continue;
       }
     }
@@ -163,9 +195,10 @@ __global__ void __launch_bounds__(256)
       float amax = 0.f;
       bool odd = false;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        amax = fmaxf(amax, fmaxf(fabsf(a[i]), fabsf(z[i])));
-        odd |= !(fabsf(a[i]) < INFINITY) || !(fabsf(z[i]) < INFINITY);
+      for (int i = 0; i < 2; ++i) {
+        const float v[4] = {a[i].x, a[i].y, z[i].x, z[i].y};
+#pragma unroll
+        for (int x = 0; x < 4; ++x) amax = fmaxf(amax, fabsf(v[x])), odd |= !(fabsf(v[x]) < INFINITY);
       }
 #pragma unroll
       for (int o = 8; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(half, amax, o));
@@ -177,9 +210,9 @@ __global__ void __launch_bounds__(256)
         s = __int_as_float(0x7fc00000);  // a row with a NaN or an infinity is kept as NaN
       } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          lo |= code(a[i], inv) << (8 * i);
-          hi |= code(z[i], inv) << (8 * i);
+        for (int i = 0; i < 2; ++i) {
+          lo |= (code(a[i].x, inv) | code(a[i].y, inv) << 8) << (16 * i);
+          hi |= (code(z[i].x, inv) | code(z[i].y, inv) << 8) << (16 * i);
         }
       }
       uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<int8_t*>(const_cast<void*>(is_k ? p.k : p.v)) + row * D);
@@ -256,11 +289,14 @@ __global__ void __launch_bounds__(256)
 template <typename T>
 static dial_status append_t(const void* qkv, const RopeArgs& r, const PagedView& p, int format, void* q_out,
                             int hq, cudaStream_t st) {
-  // few tokens: 16 heads a CTA, for latency; otherwise a CTA per token
-  const dim3 grid((unsigned)p.tokens, p.tokens < 2 * sm_count() ? (unsigned)((hq + 2 * p.hkv + 15) / 16) : 1u);
+  const int most = (hq + 2 * p.hkv + 1) / 2;  // a half-warp per head
+  const int wpt = (int)std::min<int64_t>(most, std::max<int64_t>(2, 32 * (int64_t)sm_count() / p.tokens));
+  const int64_t blocks = (p.tokens * wpt + 7) / 8;
+  if (blocks >= (1ll << 31)) return fail(DIAL_ERR_SHAPE, "too many tokens (%lld)", (long long)p.tokens);
+  const dim3 grid((unsigned)blocks);
   auto k = format == DIAL_KV_INT8 ? paged_append_kernel<T, true> : paged_append_kernel<T, false>;
   return launch_pdl("paged_append_kernel", k, grid, dim3(256), 0, st, static_cast<const T*>(qkv), r, p,
-                    static_cast<T*>(q_out), hq);
+                    static_cast<T*>(q_out), hq, wpt);
 }
 
 dial_status launch_paged_append(const void* qkv, const RopeArgs& r, const PagedView& p, int format,
