@@ -964,6 +964,20 @@ dial_status make_byte_map(CUtensorMap* map, const void* base, int64_t rows, int6
   return DIAL_OK;
 }
 
+dial_status make_halves_map(CUtensorMap* map, const void* base, int64_t rows, int box_rows) {
+  EncodeTiledFn enc = encode_fn();
+  if (!enc) return fail(DIAL_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
+  const cuuint64_t dims[3] = {128, (cuuint64_t)rows, 2};
+  const cuuint64_t strides[2] = {256, 128};
+  const cuuint32_t box[3] = {128, (cuuint32_t)box_rows, 2};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, estr,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(DIAL_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+  return DIAL_OK;
+}
+
 dial_status make_head_map(CUtensorMap* map, const void* base, int64_t tokens, int heads, int box_heads,
                           int box_tokens) {
   EncodeTiledFn enc = encode_fn();

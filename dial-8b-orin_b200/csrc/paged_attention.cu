@@ -7,17 +7,22 @@
 // bound by the bytes of the cache.
 //
 // A CTA takes a share of the key tiles of one (sequence, kv head); its four warps
-// take tiles in turn, each through a ring of its own of three 8 KB stages that one
-// lane fills by TMA (SWIZZLE_128B boxes of at most 16 or 32 rows of a page) -- 192 KB
-// in flight on an SM with its two CTAs.  Scores and P V run on mma.sync m16n8k16,
-// which these few rows do not need more of.
+// take tiles in turn, each through a ring of its own of 8 KB stages that one lane
+// fills by TMA (SWIZZLE_128B, boxes inside a page).  mma.sync m16n8k16 does the
+// products, with the query rows on its N side, eight to a tile, so that few rows
+// waste little:
+//   S^T [16 keys x 8 rows] = K Q^T,   O^T [16 dims x 8 rows] += V^T P^T;
+// S^T's 8 x 8 blocks become P^T's operand by movmatrix.  A row's maximum in use
+// moves only when a score passes it by 2^8 (a vote; the exchange over the lanes is
+// rare), and P stays below 2^8.
 //   16-bit pages: 16 keys a tile, operands by ldmatrix (V transposed).
-//   int8 pages: 32 keys a tile, widened in registers.  The order of the 128 dims in
-//   Q K^T is free as long as Q follows it: a lane takes 16 consecutive bytes of a key,
-//   so two 16-byte loads a key feed 8 k-steps; V's 4 x 4 byte blocks are transposed
-//   with byte permutes, and the dims of O come out permuted.  Scales as in
-//   paged_attention_tiles.cu: k_s on the score, log2 v_s in the exponent, 1 / v_s in
-//   the row sum.
+//   int8 pages: 32 keys a tile, widened to f16 in registers.  The order of the 128
+//   dims in K Q^T is free as long as Q follows it: a lane takes 16 consecutive bytes
+//   of a key, so two 16-byte loads a key feed 8 k-steps; V's 4 x 4 byte blocks are
+//   transposed with byte permutes, and the dims of O come out permuted.  bf16 queries
+//   become f16 times one power of two for all rows, chosen by their largest value: 34
+//   bits below it are kept.  Scales as in paged_attention_tiles.cu: k_s on the score,
+//   log2 v_s in the exponent, 1 / v_s in the row sum.
 // The warps' (m, l, O) meet in shared memory, the CTAs' in the cluster's: no
 // workspace, no counters, and the same result whatever the timing.
 #include <cuda.h>
@@ -37,10 +42,17 @@ using namespace tma;
 
 constexpr int D = 128;
 constexpr int WARPS = 4;
-constexpr int STAGES = 3;
 constexpr int TILE = 4096;            // bytes of a K or V tile
 constexpr int STAGE = 2 * TILE;
-constexpr int RING = WARPS * STAGES * STAGE;
+
+// Per 8-row tile count: stages of a warp's ring and CTAs an SM (192 KB in flight on it
+// either way).
+template <int NR>
+struct Cfg {
+  static constexpr int STAGES = NR == 1 ? 2 : 3;
+  static constexpr int PER_SM = NR == 1 ? 3 : 2;
+  static constexpr int RING = WARPS * STAGES * STAGE;
+};
 
 struct Args {
   PagedView p;
@@ -84,15 +96,23 @@ __device__ __forceinline__ float4 ld_cluster16(uint32_t addr) {
   return v;
 }
 
-// MT: 16-row tiles of query rows (rows of the chunk = token * rep + head)
-template <typename T, bool Q8, int MT>
-__global__ void __launch_bounds__(WARPS * 32, 2)
+// an 8 x 8 matrix of 16-bit values, transposed across the warp
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+// NR: 8-row tiles of query rows (rows of the chunk = token * rep + head)
+template <typename T, bool Q8, int NR>
+__global__ void __launch_bounds__(WARPS * 32, Cfg<NR>::PER_SM)
     paged_attention_rows_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
                                 const Args a) {
   constexpr int TK = Q8 ? 32 : 16;  // keys per tile
-  constexpr int NT = TK / 8;        // 8-key column tiles of the scores
-  constexpr int ROWS = 16 * MT;
-  using PT = typename std::conditional<Q8, __half, T>::type;
+  constexpr int KT = TK / 16;       // 16-key tiles of the scores
+  constexpr int ROWS = 8 * NR, STAGES = Cfg<NR>::STAGES;
+  constexpr float kGrow = 8.f;      // log2 growth of a row's maximum before it moves
+  using MT = typename std::conditional<Q8, __half, T>::type;  // operands
   extern __shared__ uint8_t smem_raw[];
   __shared__ float sm_m[WARPS][ROWS], sm_l[WARPS][ROWS], cta_m[ROWS], cta_l[ROWS];
   __shared__ __align__(8) uint64_t bars[WARPS * STAGES];
@@ -119,203 +139,238 @@ __global__ void __launch_bounds__(WARPS * 32, 2)
   const int len = ch.n > 0 ? ch.kv : 0;
   const int ntile = (len + TK - 1) / TK;
   const int t0 = (int)((int64_t)ntile * rank / S), t1 = (int)((int64_t)ntile * (rank + 1) / S);
-  const int page = 1 << a.p.log2_page;
+  const int mine = t0 + warp;                          // this warp's tiles: mine + i WARPS
+  const int box = min(1 << a.p.log2_page, TK);
 
-  auto fetch = [&](int tile, int st) {  // by lane 0
-    const int k0 = tile * TK;
-    const uint32_t dst = ring + st * STAGE, fb = bar + 8 * st;
-    if constexpr (Q8) {
-      const int box = min(page, TK), n = min(TK / box, (ch.kv - k0 + box - 1) / box);
-      mbar_expect_tx(fb, (uint32_t)(2 * n * box * 128));
-      for (int x = 0; x < n; ++x) {
-        const int row = (int)pool_row(a.p, b, g, k0 + x * box);
-        load_2d(dst + x * box * 128, &kmap, fb, 0, row);
-        load_2d(dst + TILE + x * box * 128, &vmap, fb, 0, row);
-      }
-    } else {
-      const int row = (int)pool_row(a.p, b, g, k0);
-      mbar_expect_tx(fb, STAGE);
-      load_2d(dst, &kmap, fb, 0, row);
-      load_2d(dst + TILE / 2, &kmap, fb, 128, row);
-      load_2d(dst + TILE, &vmap, fb, 0, row);
-      load_2d(dst + TILE + TILE / 2, &vmap, fb, 128, row);
+  // pool rows of this warp's tiles, 32 tiles at a time, a lane each (two for an int8 tile
+  // over two 16-row pages)
+  int row0 = 0, row1 = 0;
+  auto look_up = [&](int i) {  // for tiles i .. i + 31 of this warp
+    const int k = (mine + (i + lane) * WARPS) * TK;
+    if (mine + (i + lane) * WARPS < t1) {
+      row0 = (int)pool_row(a.p, b, g, k);
+      if (Q8 && box < TK && k + box < ch.kv) row1 = (int)pool_row(a.p, b, g, k + box);
     }
   };
-  if (lane == 0)
-    for (int s = 0; s < STAGES; ++s)
-      if (t0 + warp + s * WARPS < t1) fetch(t0 + warp + s * WARPS, s);
-
-  // scales of this lane's key of a tile (int8)
-  float ks = 0.f, vs = 1.f;
-  auto scales = [&](int tile) {
-    const int key = tile * TK + lane;
-    ks = 0.f, vs = 1.f;
-    if (key < ch.kv) {
-      const int64_t r = pool_row(a.p, b, g, key);
-      ks = __ldg(a.p.ks + r);
-      vs = __ldg(a.p.vs + r);
-    }
-  };
-  if (Q8 && t0 + warp < t1) scales(t0 + warp);
-
-  // Q fragments: rows g8 and g8 + 8 of each row tile; k-step s
-  uint32_t qa[MT][8][4];
-#pragma unroll
-  for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-    for (int hf = 0; hf < 2; ++hf) {
-      const int r = 16 * mt + 8 * hf + g8, i = r / a.rep;
-      const bool in = i < ch.n;
-      const T* src = static_cast<const T*>(a.q) + ((ch.q0 + (in ? i : 0)) * a.hq + g * a.rep + r % a.rep) * D;
-#pragma unroll
-      for (int s = 0; s < 8; ++s) {
-        if constexpr (Q8) {  // dims 32 qd + 4 s .. + 3
-          const uint2 w = in ? __ldg(reinterpret_cast<const uint2*>(src + 32 * qd + 4 * s)) : make_uint2(0, 0);
-          qa[mt][s][hf] = w.x;
-          qa[mt][s][2 + hf] = w.y;
-        } else {  // dims 16 s + 2 qd, + 1 and 8 further on
-          qa[mt][s][hf] = in ? __ldg(reinterpret_cast<const uint32_t*>(src + 16 * s + 2 * qd)) : 0u;
-          qa[mt][s][2 + hf] = in ? __ldg(reinterpret_cast<const uint32_t*>(src + 16 * s + 8 + 2 * qd)) : 0u;
+  auto fetch = [&](int i, int st) {  // tile i of this warp (the whole warp calls)
+    const int r0 = __shfl_sync(0xffffffffu, row0, i & 31), r1 = __shfl_sync(0xffffffffu, row1, i & 31);
+    if (lane == 0) {
+      const uint32_t dst = ring + st * STAGE, fb = bar + 8 * st;
+      if constexpr (Q8) {
+        const bool both = box < TK && (mine + i * WARPS) * TK + box < ch.kv;
+        mbar_expect_tx(fb, (uint32_t)(2 * (both ? TK : box) * 128));
+        load_2d(dst, &kmap, fb, 0, r0);
+        load_2d(dst + TILE, &vmap, fb, 0, r0);
+        if (both) {
+          load_2d(dst + box * 128, &kmap, fb, 0, r1);
+          load_2d(dst + TILE + box * 128, &vmap, fb, 0, r1);
         }
+      } else {
+        mbar_expect_tx(fb, STAGE);
+        load_3d(dst, &kmap, fb, 0, r0, 0);
+        load_3d(dst + TILE, &vmap, fb, 0, r0, 0);
       }
     }
+    __syncwarp();
+  };
+  const int count = mine < t1 ? (t1 - mine + WARPS - 1) / WARPS : 0;
+  look_up(0);
+  for (int s = 0; s < STAGES; ++s)
+    if (s < count) fetch(s, s);
 
-  float m[MT][2], l[MT][2], o[MT][16][4];
-  int lim[MT][2];
+  // scales of this lane's keys of a tile (int8): g8 + 8 x
+  float ks[2 * KT], vs[2 * KT];
+  auto scales = [&](int tile) {
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt) {
+    for (int x = 0; x < 2 * KT; ++x) {
+      const int key = tile * TK + 8 * x + g8;
+      ks[x] = 0.f, vs[x] = 1.f;
+      if (key < ch.kv) {
+        const int64_t r = pool_row(a.p, b, g, key);
+        ks[x] = __ldg(a.p.ks + r);
+        vs[x] = __ldg(a.p.vs + r);
+      }
+    }
+  };
+  if (Q8 && count) scales(mine);
+
+  // Q: row 8 n + g8; k-step s
+  uint32_t qb[NR][8][2];
 #pragma unroll
-    for (int hf = 0; hf < 2; ++hf) {
-      const int i = (16 * mt + 8 * hf + g8) / a.rep;
-      m[mt][hf] = -INFINITY;
-      l[mt][hf] = 0.f;
-      lim[mt][hf] = i < ch.n ? before + i + 1 : 0;
+  for (int n = 0; n < NR; ++n) {
+    const int r = 8 * n + g8, i = r / a.rep;
+    const bool in = i < ch.n;
+    const T* src = static_cast<const T*>(a.q) + ((ch.q0 + (in ? i : 0)) * a.hq + g * a.rep + r % a.rep) * D;
+#pragma unroll
+    for (int s = 0; s < 8; ++s) {
+      if constexpr (Q8) {  // dims 32 qd + 4 s .. + 3
+        const uint2 w = in ? __ldg(reinterpret_cast<const uint2*>(src + 32 * qd + 4 * s)) : make_uint2(0, 0);
+        qb[n][s][0] = w.x;
+        qb[n][s][1] = w.y;
+      } else {  // dims 16 s + 2 qd, + 1 and 8 further on
+        qb[n][s][0] = in ? __ldg(reinterpret_cast<const uint32_t*>(src + 16 * s + 2 * qd)) : 0u;
+        qb[n][s][1] = in ? __ldg(reinterpret_cast<const uint32_t*>(src + 16 * s + 8 + 2 * qd)) : 0u;
+      }
+    }
+  }
+  float c = a.c;
+  if constexpr (Q8 && std::is_same<T, __nv_bfloat16>::value) {  // to f16, the largest to 2^10 .. 2^11
+    float top = 0.f;
+    auto lo = [](uint32_t w) { return __uint_as_float(w << 16); };
+    auto hi = [](uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); };
+#pragma unroll
+    for (int n = 0; n < NR; ++n)
+#pragma unroll
+      for (int s = 0; s < 8; ++s)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float x = fabsf(lo(qb[n][s][e])), y = fabsf(hi(qb[n][s][e]));
+          if (x < INFINITY) top = fmaxf(top, x);
+          if (y < INFINITY) top = fmaxf(top, y);
+        }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const int e = min(max((int)(__float_as_uint(top) >> 23) - 127 - 10, -100), 100);
+    const float down = __uint_as_float((uint32_t)(127 - e) << 23);
+    c *= __uint_as_float((uint32_t)(127 + e) << 23);
+#pragma unroll
+    for (int n = 0; n < NR; ++n)
+#pragma unroll
+      for (int s = 0; s < 8; ++s)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) qb[n][s][x] = pack2<__half>(lo(qb[n][s][x]) * down, hi(qb[n][s][x]) * down);
+  }
+
+  float m[NR][2], l[NR][2], o[NR][8][4];  // rows 8 n + 2 qd, + 1
+  int lim[NR][2];
+#pragma unroll
+  for (int n = 0; n < NR; ++n) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int i = (8 * n + 2 * qd + e) / a.rep;
+      m[n][e] = -INFINITY;
+      l[n][e] = 0.f;
+      lim[n][e] = i < ch.n ? before + i + 1 : 0;
     }
 #pragma unroll
-    for (int n = 0; n < 16; ++n) o[mt][n][0] = o[mt][n][1] = o[mt][n][2] = o[mt][n][3] = 0.f;
+    for (int x = 0; x < 8; ++x) o[n][x][0] = o[n][x][1] = o[n][x][2] = o[n][x][3] = 0.f;
   }
 
   const int mi = lane >> 3, ri = lane & 7;
   int st = 0;
   uint32_t ph = 0;
-  for (int tile = t0 + warp; tile < t1; tile += WARPS) {
+  for (int i = 0; i < count; ++i) {
+    const int tile = mine + i * WARPS, k0 = tile * TK;
     if (!__all_sync(0xffffffffu, wait(bar + 8 * st, ph, err))) break;
     const uint32_t kt = ring + st * STAGE, vt = kt + TILE;
-    const int k0 = tile * TK;
-    float sc[MT][NT][4];
+    float sc[NR][KT][4];  // keys 16 x + g8 (0, 1) and + 8 (2, 3), rows 2 qd, + 1
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
+    for (int n = 0; n < NR; ++n)
 #pragma unroll
-      for (int n = 0; n < NT; ++n) sc[mt][n][0] = sc[mt][n][1] = sc[mt][n][2] = sc[mt][n][3] = 0.f;
+      for (int x = 0; x < KT; ++x) sc[n][x][0] = sc[n][x][1] = sc[n][x][2] = sc[n][x][3] = 0.f;
     if constexpr (Q8) {
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        const int key = 8 * n + g8;
+      for (int x = 0; x < KT; ++x) {
+        const int key = 16 * x + g8;  // and key + 8: the same place in its group of eight
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const uint4 w = lds16(kt + key * 128 + (((2 * qd + h) ^ (key & 7)) << 4));
-          const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+          const uint32_t at = kt + key * 128 + (((2 * qd + h) ^ (key & 7)) << 4);
+          const uint4 u = lds16(at), w = lds16(at + 1024);
+          const uint32_t uu[4] = {u.x, u.y, u.z, u.w}, ww[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            uint32_t b0, b1;
-            widen<T>(ww[x], b0, b1);
+          for (int y = 0; y < 4; ++y) {
+            uint32_t f[4];
+            widen<__half>(uu[y], f[0], f[2]);
+            widen<__half>(ww[y], f[1], f[3]);
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt) mma<T>(sc[mt][n], qa[mt][4 * h + x], b0, b1);
+            for (int n = 0; n < NR; ++n) mma<MT>(sc[n][x], f, qb[n][4 * h + y][0], qb[n][4 * h + y][1]);
           }
         }
       }
     } else {
       if (k0 + TK > ch.kv) {  // value rows behind the cache's end must not meet a zero as a NaN
-        for (int i = (ch.kv - k0) * 8 + lane; i < TK * 8; i += 32) {
-          sts16(vt + i * 16, make_uint4(0, 0, 0, 0));
-          sts16(vt + TILE / 2 + i * 16, make_uint4(0, 0, 0, 0));
+        for (int x = (ch.kv - k0) * 8 + lane; x < TK * 8; x += 32) {
+          sts16(vt + x * 16, make_uint4(0, 0, 0, 0));
+          sts16(vt + TILE / 2 + x * 16, make_uint4(0, 0, 0, 0));
         }
         __syncwarp();
       }
 #pragma unroll
-      for (int s = 0; s < 8; ++s) {
-        const int row = (mi >> 1) * 8 + ri, cc = 2 * (s & 3) + (mi & 1);
-        uint32_t w[4];
-        ldsm(kt + (s >> 2) * (TILE / 2) + row * 128 + ((cc ^ (row & 7)) << 4), w);
+      for (int s = 0; s < 8; ++s) {  // keys ri and ri + 8, chunks 2 s and 2 s + 1
+        const int row = (mi & 1) * 8 + ri, cc = 2 * (s & 3) + (mi >> 1);
+        uint32_t f[4];
+        ldsm(kt + (s >> 2) * (TILE / 2) + row * 128 + ((cc ^ (row & 7)) << 4), f);
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-          mma<T>(sc[mt][0], qa[mt][s], w[0], w[1]);
-          mma<T>(sc[mt][1], qa[mt][s], w[2], w[3]);
-        }
+        for (int n = 0; n < NR; ++n) mma<MT>(sc[n][0], f, qb[n][s][0], qb[n][s][1]);
       }
     }
-    // scores in log2 units; this lane holds keys 8 n + 2 qd, + 1 of rows g8 and g8 + 8
-    float rv[NT][2];
+    // scores in log2 units, those that a row does not see at minus infinity
+    const bool masked = k0 + TK > before + 1;
+    float rv[2 * KT];
+    float kc[2 * KT], lv[2 * KT];
     if constexpr (Q8) {
-      const float kc = ks * a.c, lv = __log2f(vs), iv = 1.f / vs;
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+      for (int x = 0; x < 2 * KT; ++x) kc[x] = ks[x] * c, lv[x] = __log2f(vs[x]), rv[x] = __frcp_rn(vs[x]);
+      if (i + 1 < count) scales(tile + WARPS);
+    }
+    bool grow = false;
+#pragma unroll
+    for (int n = 0; n < NR; ++n)
+#pragma unroll
+      for (int x = 0; x < KT; ++x)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float& v = sc[n][x][e];
+          v = Q8 ? fmaf(v, kc[2 * x + (e >> 1)], lv[2 * x + (e >> 1)]) : v * c;
+          if (masked && k0 + 16 * x + 8 * (e >> 1) + g8 >= lim[n][e & 1]) v = -INFINITY;
+          grow |= v > m[n][e & 1] + kGrow;
+        }
+    if (__any_sync(0xffffffffu, grow)) {  // rare: the rows' maxima move
+#pragma unroll
+      for (int n = 0; n < NR; ++n)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const float f = __shfl_sync(0xffffffffu, kc, 8 * n + 2 * qd + e);
-          const float v = __shfl_sync(0xffffffffu, lv, 8 * n + 2 * qd + e);
-          rv[n][e] = __shfl_sync(0xffffffffu, iv, 8 * n + 2 * qd + e);
+          float mx = -INFINITY;
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt) {
-            sc[mt][n][e] = fmaf(sc[mt][n][e], f, v);
-            sc[mt][n][2 + e] = fmaf(sc[mt][n][2 + e], f, v);
-          }
+          for (int x = 0; x < KT; ++x) mx = fmaxf(mx, fmaxf(sc[n][x][e], sc[n][x][2 + e]));
+#pragma unroll
+          for (int z = 4; z < 32; z <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, z));
+          const float mn = fmaxf(m[n][e], mx);
+          const float f = m[n][e] == -INFINITY ? 0.f : ex2(m[n][e] - mn);
+          m[n][e] = mn;
+          l[n][e] *= f;
+#pragma unroll
+          for (int x = 0; x < 8; ++x) o[n][x][e] *= f, o[n][x][2 + e] *= f;
         }
-      if (tile + WARPS < t1) scales(tile + WARPS);
-    } else {
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) sc[mt][n][e] *= a.c;
     }
-    const bool masked = k0 + TK > before + 1;
-    uint32_t pa_[MT][NT / 2][4];
+    uint32_t pb[NR][KT][2];  // P^T: keys 2 qd, + 1 (and 8 further on), row g8
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
+    for (int n = 0; n < NR; ++n) {
+      const float s0 = m[n][0] == -INFINITY ? 0.f : m[n][0], s1 = m[n][1] == -INFINITY ? 0.f : m[n][1];
 #pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        float mx = -INFINITY;
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float& x = sc[mt][n][2 * hf + e];
-            if (masked && k0 + 8 * n + 2 * qd + e >= lim[mt][hf]) x = -INFINITY;
-            mx = fmaxf(mx, x);
-          }
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        const float mn = fmaxf(m[mt][hf], mx);
-        const float f = m[mt][hf] == -INFINITY ? 0.f : ex2(m[mt][hf] - mn);
-        m[mt][hf] = mn;
-        const float sub = mn == -INFINITY ? 0.f : mn;
-        float sum = 0.f;
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          const float x = ex2(sc[mt][n][2 * hf] - sub), y = ex2(sc[mt][n][2 * hf + 1] - sub);
-          if constexpr (Q8) {
-            // a key that the row does not see has no part in its sum, whatever its scale is
-            sum += masked && x == 0.f ? 0.f : x * rv[n][0];
-            sum += masked && y == 0.f ? 0.f : y * rv[n][1];
+      for (int x = 0; x < KT; ++x) {
+        float* v = sc[n][x];
+        v[0] = ex2(v[0] - s0), v[1] = ex2(v[1] - s1), v[2] = ex2(v[2] - s0), v[3] = ex2(v[3] - s1);
+        if constexpr (Q8) {
+          if (masked) {  // a key that the row does not see has no part in its sum, whatever its scale is
+            l[n][0] += (v[0] == 0.f ? 0.f : v[0] * rv[2 * x]) + (v[2] == 0.f ? 0.f : v[2] * rv[2 * x + 1]);
+            l[n][1] += (v[1] == 0.f ? 0.f : v[1] * rv[2 * x]) + (v[3] == 0.f ? 0.f : v[3] * rv[2 * x + 1]);
           } else {
-            sum += x + y;
+            l[n][0] = fmaf(v[0], rv[2 * x], fmaf(v[2], rv[2 * x + 1], l[n][0]));
+            l[n][1] = fmaf(v[1], rv[2 * x], fmaf(v[3], rv[2 * x + 1], l[n][1]));
           }
-          pa_[mt][n / 2][2 * (n & 1) + hf] = pack2<PT>(x, y);
+        } else {
+          l[n][0] += v[0] + v[2];
+          l[n][1] += v[1] + v[3];
         }
-        l[mt][hf] = l[mt][hf] * f + sum;
-#pragma unroll
-        for (int n = 0; n < 16; ++n) {
-          o[mt][n][2 * hf] *= f;
-          o[mt][n][2 * hf + 1] *= f;
-        }
+        pb[n][x][0] = transpose8(pack2<MT>(v[0], v[1]));
+        pb[n][x][1] = transpose8(pack2<MT>(v[2], v[3]));
       }
     }
-    // O += P V
+    // O^T += V^T P^T
     if constexpr (Q8) {
 #pragma unroll
-      for (int kk = 0; kk < 2; ++kk) {
+      for (int kk = 0; kk < KT; ++kk) {
         uint32_t w[4][4];
 #pragma unroll
         for (int x = 0; x < 4; ++x) {  // keys 2 qd, 2 qd + 1, 2 qd + 8, 2 qd + 9
@@ -324,68 +379,65 @@ __global__ void __launch_bounds__(WARPS * 32, 2)
           w[x][0] = u.x, w[x][1] = u.y, w[x][2] = u.z, w[x][3] = u.w;
         }
 #pragma unroll
-        for (int x = 0; x < 4; ++x)  // dims 16 g8 + 4 x .. + 3
+        for (int x = 0; x < 4; ++x)  // dims 16 g8 + 4 x .. + 3, two to a 16-dim tile
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            uint32_t b0a, b0b, b1a, b1b;
-            widen<PT>(prmt(w[0][x], w[1][x], e ? 0x7362u : 0x5140u), b0a, b0b);
-            widen<PT>(prmt(w[2][x], w[3][x], e ? 0x7362u : 0x5140u), b1a, b1b);
+            uint32_t f[4];
+            widen<__half>(prmt(w[0][x], w[1][x], e ? 0x7362u : 0x5140u), f[0], f[1]);
+            widen<__half>(prmt(w[2][x], w[3][x], e ? 0x7362u : 0x5140u), f[2], f[3]);
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-              mma<PT>(o[mt][4 * x + 2 * e], pa_[mt][kk], b0a, b1a);
-              mma<PT>(o[mt][4 * x + 2 * e + 1], pa_[mt][kk], b0b, b1b);
-            }
+            for (int n = 0; n < NR; ++n) mma<MT>(o[n][2 * x + e], f, pb[n][kk][0], pb[n][kk][1]);
           }
       }
     } else {
 #pragma unroll
-      for (int n = 0; n < 16; n += 2) {
-        const int row = (mi & 1) * 8 + ri, cc = (n + (mi >> 1)) & 7;
-        uint32_t w[4];
-        ldsm_t(vt + (n >> 3) * (TILE / 2) + row * 128 + ((cc ^ (row & 7)) << 4), w);
+      for (int x = 0; x < 8; ++x) {  // dims 16 x .. + 15: chunks 2 x (mi & 1), keys ri + 8 (mi >> 1)
+        const int row = (mi >> 1) * 8 + ri, cc = (2 * x + (mi & 1)) & 7;
+        uint32_t f[4];
+        ldsm_t(vt + (x >> 2) * (TILE / 2) + row * 128 + ((cc ^ (row & 7)) << 4), f);
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-          mma<PT>(o[mt][n], pa_[mt][0], w[0], w[1]);
-          mma<PT>(o[mt][n + 1], pa_[mt][0], w[2], w[3]);
-        }
+        for (int n = 0; n < NR; ++n) mma<MT>(o[n][x], f, pb[n][0][0], pb[n][0][1]);
       }
     }
     __syncwarp();  // every lane has read the stage
-    if (lane == 0 && tile + STAGES * WARPS < t1) fetch(tile + STAGES * WARPS, st);
+    const int next = i + STAGES;
+    if (next < count) {
+      if ((next & 31) == 0) look_up(next);
+      fetch(next, st);
+    }
     if (++st == STAGES) st = 0, ph ^= 1;
   }
 
   // ---- the warps meet: O [row][dim] in the ring, which nobody fills any more
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt)
+  for (int n = 0; n < NR; ++n)
 #pragma unroll
-    for (int hf = 0; hf < 2; ++hf) {
-      float s = l[mt][hf];
-      s += __shfl_xor_sync(0xffffffffu, s, 1);
-      s += __shfl_xor_sync(0xffffffffu, s, 2);
-      if (qd == 0) {
-        sm_m[warp][16 * mt + 8 * hf + g8] = m[mt][hf];
-        sm_l[warp][16 * mt + 8 * hf + g8] = s;
+    for (int e = 0; e < 2; ++e) {
+      float s = l[n][e];
+#pragma unroll
+      for (int z = 4; z < 32; z <<= 1) s += __shfl_xor_sync(0xffffffffu, s, z);
+      if (g8 == 0) {
+        sm_m[warp][8 * n + 2 * qd + e] = m[n][e];
+        sm_l[warp][8 * n + 2 * qd + e] = s;
       }
     }
   __syncthreads();
   const int rows = min(ROWS, ch.n * a.rep);
   float* part = reinterpret_cast<float*>(smem);  // [WARPS][rows][D]
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt)
+  for (int n = 0; n < NR; ++n)
 #pragma unroll
-    for (int hf = 0; hf < 2; ++hf) {
-      const int r = 16 * mt + 8 * hf + g8;
+    for (int e = 0; e < 2; ++e) {
+      const int r = 8 * n + 2 * qd + e;
       if (r >= rows) continue;
       float* dst = part + (warp * rows + r) * D;
 #pragma unroll
-      for (int n = 0; n < 16; ++n) {
-        const float x = o[mt][n][2 * hf], y = o[mt][n][2 * hf + 1];
-        if constexpr (Q8) {  // column 2 qd + e of tile n is dim 16 (2 qd + e) + n
-          dst[32 * qd + n] = x;
-          dst[32 * qd + 16 + n] = y;
-        } else {
-          *reinterpret_cast<float2*>(dst + 8 * n + 2 * qd) = make_float2(x, y);
+      for (int x = 0; x < 8; ++x) {
+        if constexpr (Q8) {  // dims 16 g8 + 2 x, + 1
+          *reinterpret_cast<float2*>(dst + 16 * g8 + 2 * x) = make_float2(o[n][x][e], o[n][x][2 + e]);
+        } else {             // dims 16 x + g8, + 8
+          dst[16 * x + g8] = o[n][x][e];
+          dst[16 * x + g8 + 8] = o[n][x][2 + e];
         }
       }
     }
@@ -456,38 +508,41 @@ __global__ void __launch_bounds__(WARPS * 32, 2)
   if (S > 1) cluster_sync();  // nobody leaves while another reads its part
 }
 
+#ifndef SPLIT_COST
+#define SPLIT_COST 12
+#endif
 // Key splits (CTAs of a cluster) of `units` (sequence, kv head) pairs with up to
 // `tiles` key tiles: the fewest rounds over the SMs' CTA places times the tiles a
 // warp takes, plus what a CTA costs to start and to meet the others (about 12
 // tiles of a warp).
-int key_splits(int64_t units, int64_t tiles) {
-  const int64_t places = 2 * (int64_t)sm_count();
+int key_splits(int64_t units, int64_t tiles, int per_sm) {
+  const int64_t places = per_sm * (int64_t)sm_count();
   int best = 1;
   double cost = 1e30;
   for (int s = 1; s <= 8; s *= 2) {
     if (s > 1 && tiles < 2 * WARPS * s) break;
     const double rounds = (double)((units * s + places - 1) / places);
-    const double c = rounds * ((double)tiles / (WARPS * s) + 12);
+    const double c = rounds * ((double)tiles / (WARPS * s) + SPLIT_COST);
     if (c < cost - 1e-9) cost = c, best = s;
   }
   return best;
 }
 
-template <typename T, bool Q8, int MT>
+template <typename T, bool Q8, int NR>
 dial_status launch(const void* q, const PagedView& p, void* out, int hq, int64_t max_kv, float c, cudaStream_t st) {
-  constexpr auto kern = paged_attention_rows_kernel<T, Q8, MT>;
-  constexpr int smem = RING + 1024;
+  constexpr auto kern = paged_attention_rows_kernel<T, Q8, NR>;
+  constexpr int smem = Cfg<NR>::RING + 1024;
   constexpr int TK = Q8 ? 32 : 16;
   const int64_t rows = (p.n_pages * p.hkv) << p.log2_page;
   CUtensorMap km, vm;
   const int box = std::min(1 << p.log2_page, TK);
-  dial_status s = make_byte_map(&km, p.k, rows, Q8 ? 128 : 256, 128, box, 128);
-  if (s == DIAL_OK) s = make_byte_map(&vm, p.v, rows, Q8 ? 128 : 256, 128, box, 128);
+  dial_status s = Q8 ? make_byte_map(&km, p.k, rows, 128, 128, box, 128) : make_halves_map(&km, p.k, rows, box);
+  if (s == DIAL_OK) s = Q8 ? make_byte_map(&vm, p.v, rows, 128, 128, box, 128) : make_halves_map(&vm, p.v, rows, box);
   if (s != DIAL_OK) return s;
   cudaError_t e = ensure_smem<kern>(smem);
   if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(paged_attention_rows_kernel)");
   const int64_t units = (int64_t)p.n_seqs * p.hkv;
-  const int S = key_splits(units, (max_kv + TK - 1) / TK);
+  const int S = key_splits(units, (max_kv + TK - 1) / TK, Cfg<NR>::PER_SM);
   if (units * S >= (1ll << 31)) return fail(DIAL_ERR_SHAPE, "too many sequences and heads (%lld)", (long long)units);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(units * S));
@@ -513,9 +568,12 @@ dial_status launch(const void* q, const PagedView& p, void* out, int hq, int64_t
 }
 
 template <typename T, bool Q8>
-dial_status launch_mt(const void* q, const PagedView& p, void* out, int hq, int64_t max_kv, float c, cudaStream_t st) {
-  return (int64_t)p.max_q * (hq / p.hkv) <= 16 ? launch<T, Q8, 1>(q, p, out, hq, max_kv, c, st)
-                                               : launch<T, Q8, 2>(q, p, out, hq, max_kv, c, st);
+dial_status launch_rows(const void* q, const PagedView& p, void* out, int hq, int64_t max_kv, float c, cudaStream_t st) {
+  const int64_t rows = (int64_t)p.max_q * (hq / p.hkv);
+  return rows <= 8    ? launch<T, Q8, 1>(q, p, out, hq, max_kv, c, st)
+         : rows <= 16 ? launch<T, Q8, 2>(q, p, out, hq, max_kv, c, st)
+         : rows <= 24 ? launch<T, Q8, 3>(q, p, out, hq, max_kv, c, st)
+                      : launch<T, Q8, 4>(q, p, out, hq, max_kv, c, st);
 }
 
 }  // namespace
@@ -526,9 +584,9 @@ dial_status launch_paged_attention(const void* q, const PagedView& p, int format
   const bool q8 = format == DIAL_KV_INT8;
   if ((int64_t)p.max_q * (hq / p.hkv) > 32) return launch_paged_attention_tiles(q, p, format, out, dt, hq, max_kv, c, st);
   if (dt == DIAL_F16)
-    return q8 ? launch_mt<__half, true>(q, p, out, hq, max_kv, c, st) : launch_mt<__half, false>(q, p, out, hq, max_kv, c, st);
-  return q8 ? launch_mt<__nv_bfloat16, true>(q, p, out, hq, max_kv, c, st)
-            : launch_mt<__nv_bfloat16, false>(q, p, out, hq, max_kv, c, st);
+    return q8 ? launch_rows<__half, true>(q, p, out, hq, max_kv, c, st) : launch_rows<__half, false>(q, p, out, hq, max_kv, c, st);
+  return q8 ? launch_rows<__nv_bfloat16, true>(q, p, out, hq, max_kv, c, st)
+            : launch_rows<__nv_bfloat16, false>(q, p, out, hq, max_kv, c, st);
 }
 
 }  // namespace dial

@@ -115,6 +115,9 @@ __device__ __forceinline__ void fence_barrier_init() {
 // SWIZZLE_128B, which need box_bytes == swizzle_bytes).
 dial_status make_byte_map(CUtensorMap* map, const void* base, int64_t rows, int64_t row_bytes,
                           int box_bytes, int box_rows, int swizzle_bytes);
+// 3D tensor map over [rows, 256 bytes] seen as two halves of 128 bytes: a {128 bytes,
+// box_rows, 2} box lands as [half][row][128 bytes], SWIZZLE_128B.
+dial_status make_halves_map(CUtensorMap* map, const void* base, int64_t rows, int box_rows);
 // 3D tensor map over 16-bit [tokens, heads, 128] (256-byte rows) with a {128 bytes,
 // box_heads, box_tokens} box, SWIZZLE_128B.
 dial_status make_head_map(CUtensorMap* map, const void* base, int64_t tokens, int heads, int box_heads,
