@@ -45,10 +45,10 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
 }
 
 // Row scale and reciprocal of the int8 rows: absmax / 127, 1 for rows without
-// a usable absmax (below 1e-36 its reciprocal would overflow: the codes are
-// zeros, off by less than 1e-36).
+// a usable absmax (below 1e-30, where scales and reciprocals near the ends of
+// f32's range: the codes are zeros, off by less than 1e-30).
 __device__ __forceinline__ void row_scale(float amax, float& s, float& inv) {
-  s = amax >= 1e-36f ? __fdiv_rn(amax, 127.0f) : 1.0f;
+  s = amax >= 1e-30f ? __fdiv_rn(amax, 127.0f) : 1.0f;
   inv = __fdiv_rn(1.0f, s);
 }
 // round(x / s), halves away from zero, clamped to +-127

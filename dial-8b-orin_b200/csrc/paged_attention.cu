@@ -143,13 +143,13 @@ __global__ void __launch_bounds__(WARPS * 32, Cfg<NR>::PER_SM)
   const int box = min(1 << a.p.log2_page, TK);
 
   // pool rows of this warp's tiles, 32 tiles at a time, a lane each (two for an int8 tile
-  // over two 16-row pages)
-  int row0 = 0, row1 = 0;
-  auto look_up = [&](int i) {  // for tiles i .. i + 31 of this warp
+  // over two 16-row pages): for the copies, and for the scales, which are behind them
+  int row0 = 0, row1 = 0, srow0 = 0, srow1 = 0;
+  auto look_up = [&](int i, int& r0, int& r1) {  // tiles i .. i + 31 of this warp
     const int k = (mine + (i + lane) * WARPS) * TK;
     if (mine + (i + lane) * WARPS < t1) {
-      row0 = (int)pool_row(a.p, b, g, k);
-      if (Q8 && box < TK && k + box < ch.kv) row1 = (int)pool_row(a.p, b, g, k + box);
+      r0 = (int)pool_row(a.p, b, g, k);
+      if (Q8 && box < TK && k + box < ch.kv) r1 = (int)pool_row(a.p, b, g, k + box);
     }
   };
   auto fetch = [&](int i, int st) {  // tile i of this warp (the whole warp calls)
@@ -174,25 +174,27 @@ __global__ void __launch_bounds__(WARPS * 32, Cfg<NR>::PER_SM)
     __syncwarp();
   };
   const int count = mine < t1 ? (t1 - mine + WARPS - 1) / WARPS : 0;
-  look_up(0);
+  look_up(0, row0, row1);
+  srow0 = row0, srow1 = row1;
   for (int s = 0; s < STAGES; ++s)
     if (s < count) fetch(s, s);
 
-  // scales of this lane's keys of a tile (int8): g8 + 8 x
+  // scales of this lane's keys of tile i (int8): g8 + 8 x.  Rows behind the cache's end are
+  // in the same page, and masked.
   float ks[2 * KT], vs[2 * KT];
-  auto scales = [&](int tile) {
+  auto scales = [&](int i) {
+    if ((i & 31) == 0 && i) look_up(i, srow0, srow1);
+    const int r0 = __shfl_sync(0xffffffffu, srow0, i & 31), r1 = __shfl_sync(0xffffffffu, srow1, i & 31);
+    const bool both = box == TK || (mine + i * WARPS) * TK + box < ch.kv;
 #pragma unroll
     for (int x = 0; x < 2 * KT; ++x) {
-      const int key = tile * TK + 8 * x + g8;
-      ks[x] = 0.f, vs[x] = 1.f;
-      if (key < ch.kv) {
-        const int64_t r = pool_row(a.p, b, g, key);
-        ks[x] = __ldg(a.p.ks + r);
-        vs[x] = __ldg(a.p.vs + r);
-      }
+      const int r = x < KT || box == TK ? r0 + 8 * x + g8 : r1 + 8 * (x - KT) + g8;
+      const bool in = x < KT || both;
+      ks[x] = in ? __ldg(a.p.ks + r) : 0.f;
+      vs[x] = in ? __ldg(a.p.vs + r) : 1.f;
     }
   };
-  if (Q8 && count) scales(mine);
+  if (Q8 && count) scales(0);
 
   // Q: row 8 n + g8; k-step s
   uint32_t qb[NR][8][2];
@@ -304,27 +306,41 @@ __global__ void __launch_bounds__(WARPS * 32, Cfg<NR>::PER_SM)
         for (int n = 0; n < NR; ++n) mma<MT>(sc[n][0], f, qb[n][s][0], qb[n][s][1]);
       }
     }
-    // scores in log2 units, those that a row does not see at minus infinity
+    // scores in log2 units (16-bit pages: before the factor c), those that a row does not see
+    // at minus infinity
     const bool masked = k0 + TK > before + 1;
     float rv[2 * KT];
-    float kc[2 * KT], lv[2 * KT];
     if constexpr (Q8) {
 #pragma unroll
-      for (int x = 0; x < 2 * KT; ++x) kc[x] = ks[x] * c, lv[x] = __log2f(vs[x]), rv[x] = __frcp_rn(vs[x]);
-      if (i + 1 < count) scales(tile + WARPS);
+      for (int x = 0; x < 2 * KT; ++x) {
+        const float kc = ks[x] * c, lv = lg2(vs[x]);
+        rv[x] = rcp(vs[x]);
+#pragma unroll
+        for (int n = 0; n < NR; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) sc[n][x / 2][2 * (x & 1) + e] = fmaf(sc[n][x / 2][2 * (x & 1) + e], kc, lv);
+      }
+      if (i + 1 < count) scales(i + 1);
+    }
+    if (masked) {
+#pragma unroll
+      for (int n = 0; n < NR; ++n)
+#pragma unroll
+        for (int x = 0; x < KT; ++x)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (k0 + 16 * x + 8 * (e >> 1) + g8 >= lim[n][e & 1]) sc[n][x][e] = -INFINITY;
     }
     bool grow = false;
 #pragma unroll
     for (int n = 0; n < NR; ++n)
 #pragma unroll
-      for (int x = 0; x < KT; ++x)
+      for (int e = 0; e < 2; ++e) {
+        float mx = fmaxf(sc[n][0][e], sc[n][0][2 + e]);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float& v = sc[n][x][e];
-          v = Q8 ? fmaf(v, kc[2 * x + (e >> 1)], lv[2 * x + (e >> 1)]) : v * c;
-          if (masked && k0 + 16 * x + 8 * (e >> 1) + g8 >= lim[n][e & 1]) v = -INFINITY;
-          grow |= v > m[n][e & 1] + kGrow;
-        }
+        for (int x = 1; x < KT; ++x) mx = fmaxf(mx, fmaxf(sc[n][x][e], sc[n][x][2 + e]));
+        grow |= (Q8 ? mx : mx * c) > m[n][e] + kGrow;
+      }
     if (__any_sync(0xffffffffu, grow)) {  // rare: the rows' maxima move
 #pragma unroll
       for (int n = 0; n < NR; ++n)
@@ -335,7 +351,7 @@ __global__ void __launch_bounds__(WARPS * 32, Cfg<NR>::PER_SM)
           for (int x = 0; x < KT; ++x) mx = fmaxf(mx, fmaxf(sc[n][x][e], sc[n][x][2 + e]));
 #pragma unroll
           for (int z = 4; z < 32; z <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, z));
-          const float mn = fmaxf(m[n][e], mx);
+          const float mn = fmaxf(m[n][e], Q8 ? mx : mx * c);
           const float f = m[n][e] == -INFINITY ? 0.f : ex2(m[n][e] - mn);
           m[n][e] = mn;
           l[n][e] *= f;
@@ -350,7 +366,10 @@ __global__ void __launch_bounds__(WARPS * 32, Cfg<NR>::PER_SM)
 #pragma unroll
       for (int x = 0; x < KT; ++x) {
         float* v = sc[n][x];
-        v[0] = ex2(v[0] - s0), v[1] = ex2(v[1] - s1), v[2] = ex2(v[2] - s0), v[3] = ex2(v[3] - s1);
+        if constexpr (Q8)
+          v[0] = ex2(v[0] - s0), v[1] = ex2(v[1] - s1), v[2] = ex2(v[2] - s0), v[3] = ex2(v[3] - s1);
+        else
+          v[0] = ex2(fmaf(v[0], c, -s0)), v[1] = ex2(fmaf(v[1], c, -s1)), v[2] = ex2(fmaf(v[2], c, -s0)), v[3] = ex2(fmaf(v[3], c, -s1));
         if constexpr (Q8) {
           if (masked) {  // a key that the row does not see has no part in its sum, whatever its scale is
             l[n][0] += (v[0] == 0.f ? 0.f : v[0] * rv[2 * x]) + (v[2] == 0.f ? 0.f : v[2] * rv[2 * x + 1]);
@@ -402,7 +421,7 @@ __global__ void __launch_bounds__(WARPS * 32, Cfg<NR>::PER_SM)
     __syncwarp();  // every lane has read the stage
     const int next = i + STAGES;
     if (next < count) {
-      if ((next & 31) == 0) look_up(next);
+      if ((next & 31) == 0) look_up(next, row0, row1);
       fetch(next, st);
     }
     if (++st == STAGES) st = 0, ph ^= 1;

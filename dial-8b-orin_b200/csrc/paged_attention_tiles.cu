@@ -334,8 +334,8 @@ __global__ void __launch_bounds__(Cfg<Q8>::THREADS, 1)
           float* sc = reinterpret_cast<float*>(smem + L::SC_OFF) + (j % 3) * 3 * KT;
           const bool in = (j0 + j) * KT + row < ch.kv;
           sc[row] = ks * a.c;
-          sc[KT + row] = in ? __log2f(vs) : 0.f;
-          sc[2 * KT + row] = in ? 1.f / vs : 0.f;
+          sc[KT + row] = in ? lg2(vs) : 0.f;
+          sc[2 * KT + row] = in ? rcp(vs) : 0.f;
           if (j + 1 < nj) scales(j + 1);
         }
         const uint32_t src = base + L::RAW_OFF + (u % 3) * RAW + row * 128;

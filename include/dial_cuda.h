@@ -465,7 +465,7 @@ typedef struct dial_rope_axes {
  * from cos_t / sin_t [table_rows, 64] f32 (dial_rope_tables with DIAL_F32) at
  * positions [n_axes, T]; q goes to q_out [T, Hq, 128], k and v to the tokens' cache
  * rows.  f32 arithmetic, one rounding to dt -- or, for DIAL_KV_INT8, scale =
- * absmax / 127 (1 for an all-zero row) and code = round(x * (1 / scale)), halves
+ * absmax / 127 (1 for a row below 1e-30) and code = round(x * (1 / scale)), halves
  * away from zero, as dial_w8a16_quantize; a row with a NaN or an infinity is kept
  * as NaN.  A position outside the table sets the device error flag and uses its
  * nearest row.  Two tokens of one call must not share a cache row. */
