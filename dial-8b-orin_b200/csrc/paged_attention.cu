@@ -41,16 +41,15 @@ using namespace pa;
 using namespace tma;
 
 constexpr int D = 128;
-constexpr int WARPS = 4;
-constexpr int TILE = 4096;            // bytes of a K or V tile
-constexpr int STAGE = 2 * TILE;
-
-// Per 8-row tile count: stages of a warp's ring and CTAs an SM (192 KB in flight on it
-// either way).
-template <int NR>
+// A CTA's warps, their rings and how many CTAs share an SM (about 192 KB in flight on it).
+template <bool Q8, int NR>
 struct Cfg {
-  static constexpr int STAGES = NR == 1 ? 2 : 3;
-  static constexpr int PER_SM = NR == 1 ? 3 : 2;
+  static constexpr int WARPS = Q8 && NR == 1 ? 8 : 4;
+  static constexpr int TK = Q8 && NR > 1 ? 32 : 16;  // keys per tile
+  static constexpr int TILE = TK * (Q8 ? 128 : 256); // bytes of a K or V tile
+  static constexpr int STAGE = 2 * TILE;
+  static constexpr int STAGES = !Q8 && NR == 1 ? 2 : 3;
+  static constexpr int PER_SM = !Q8 && NR == 1 ? 3 : 2;
   static constexpr int RING = WARPS * STAGES * STAGE;
 };
 
@@ -105,12 +104,13 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
 
 // NR: 8-row tiles of query rows (rows of the chunk = token * rep + head)
 template <typename T, bool Q8, int NR>
-__global__ void __launch_bounds__(WARPS * 32, Cfg<NR>::PER_SM)
+__global__ void __launch_bounds__((Cfg<Q8, NR>::WARPS * 32), (Cfg<Q8, NR>::PER_SM))
     paged_attention_rows_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
                                 const Args a) {
-  constexpr int TK = Q8 ? 32 : 16;  // keys per tile
+  using L = Cfg<Q8, NR>;
+  constexpr int TK = L::TK, WARPS = L::WARPS, TILE = L::TILE, STAGE = L::STAGE, STAGES = L::STAGES;
   constexpr int KT = TK / 16;       // 16-key tiles of the scores
-  constexpr int ROWS = 8 * NR, STAGES = Cfg<NR>::STAGES;
+  constexpr int ROWS = 8 * NR;
   constexpr float kGrow = 8.f;      // log2 growth of a row's maximum before it moves
   using MT = typename std::conditional<Q8, __half, T>::type;  // operands
   extern __shared__ uint8_t smem_raw[];
@@ -534,7 +534,7 @@ __global__ void __launch_bounds__(WARPS * 32, Cfg<NR>::PER_SM)
 // `tiles` key tiles: the fewest rounds over the SMs' CTA places times the tiles a
 // warp takes, plus what a CTA costs to start and to meet the others (about 12
 // tiles of a warp).
-int key_splits(int64_t units, int64_t tiles, int per_sm) {
+int key_splits(int64_t units, int64_t tiles, int per_sm, int WARPS) {
   const int64_t places = per_sm * (int64_t)sm_count();
   int best = 1;
   double cost = 1e30;
@@ -550,8 +550,8 @@ int key_splits(int64_t units, int64_t tiles, int per_sm) {
 template <typename T, bool Q8, int NR>
 dial_status launch(const void* q, const PagedView& p, void* out, int hq, int64_t max_kv, float c, cudaStream_t st) {
   constexpr auto kern = paged_attention_rows_kernel<T, Q8, NR>;
-  constexpr int smem = Cfg<NR>::RING + 1024;
-  constexpr int TK = Q8 ? 32 : 16;
+  using L = Cfg<Q8, NR>;
+  constexpr int smem = L::RING + 1024, TK = L::TK;
   const int64_t rows = (p.n_pages * p.hkv) << p.log2_page;
   CUtensorMap km, vm;
   const int box = std::min(1 << p.log2_page, TK);
@@ -561,11 +561,11 @@ dial_status launch(const void* q, const PagedView& p, void* out, int hq, int64_t
   cudaError_t e = ensure_smem<kern>(smem);
   if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(paged_attention_rows_kernel)");
   const int64_t units = (int64_t)p.n_seqs * p.hkv;
-  const int S = key_splits(units, (max_kv + TK - 1) / TK, Cfg<NR>::PER_SM);
+  const int S = key_splits(units, (max_kv + TK - 1) / TK, L::PER_SM, L::WARPS);
   if (units * S >= (1ll << 31)) return fail(DIAL_ERR_SHAPE, "too many sequences and heads (%lld)", (long long)units);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(units * S));
-  cfg.blockDim = dim3(WARPS * 32);
+  cfg.blockDim = dim3(L::WARPS * 32);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute at[2];
