@@ -142,6 +142,26 @@ __global__ void __launch_bounds__((Cfg<Q8, NR>::WARPS * 32), (Cfg<Q8, NR>::PER_S
   const int mine = t0 + warp;                          // this warp's tiles: mine + i WARPS
   const int box = min(1 << a.p.log2_page, TK);
 
+  // Q: row 8 n + g8; k-step s (asked for before the tiles, which would keep it waiting)
+  uint32_t qb[NR][8][2];
+#pragma unroll
+  for (int n = 0; n < NR; ++n) {
+    const int r = 8 * n + g8, i = r / a.rep;
+    const bool in = i < ch.n;
+    const T* src = static_cast<const T*>(a.q) + ((ch.q0 + (in ? i : 0)) * a.hq + g * a.rep + r % a.rep) * D;
+#pragma unroll
+    for (int s = 0; s < 8; ++s) {
+      if constexpr (Q8) {  // dims 32 qd + 4 s .. + 3
+        const uint2 w = in ? __ldg(reinterpret_cast<const uint2*>(src + 32 * qd + 4 * s)) : make_uint2(0, 0);
+        qb[n][s][0] = w.x;
+        qb[n][s][1] = w.y;
+      } else {  // dims 16 s + 2 qd, + 1 and 8 further on
+        qb[n][s][0] = in ? __ldg(reinterpret_cast<const uint32_t*>(src + 16 * s + 2 * qd)) : 0u;
+        qb[n][s][1] = in ? __ldg(reinterpret_cast<const uint32_t*>(src + 16 * s + 8 + 2 * qd)) : 0u;
+      }
+    }
+  }
+
   // pool rows of this warp's tiles, 32 tiles at a time, a lane each (two for an int8 tile
   // over two 16-row pages): for the copies, and for the scales, which are behind them
   int row0 = 0, row1 = 0, srow0 = 0, srow1 = 0;
@@ -196,25 +216,6 @@ __global__ void __launch_bounds__((Cfg<Q8, NR>::WARPS * 32), (Cfg<Q8, NR>::PER_S
   };
   if (Q8 && count) scales(0);
 
-  // Q: row 8 n + g8; k-step s
-  uint32_t qb[NR][8][2];
-#pragma unroll
-  for (int n = 0; n < NR; ++n) {
-    const int r = 8 * n + g8, i = r / a.rep;
-    const bool in = i < ch.n;
-    const T* src = static_cast<const T*>(a.q) + ((ch.q0 + (in ? i : 0)) * a.hq + g * a.rep + r % a.rep) * D;
-#pragma unroll
-    for (int s = 0; s < 8; ++s) {
-      if constexpr (Q8) {  // dims 32 qd + 4 s .. + 3
-        const uint2 w = in ? __ldg(reinterpret_cast<const uint2*>(src + 32 * qd + 4 * s)) : make_uint2(0, 0);
-        qb[n][s][0] = w.x;
-        qb[n][s][1] = w.y;
-      } else {  // dims 16 s + 2 qd, + 1 and 8 further on
-        qb[n][s][0] = in ? __ldg(reinterpret_cast<const uint32_t*>(src + 16 * s + 2 * qd)) : 0u;
-        qb[n][s][1] = in ? __ldg(reinterpret_cast<const uint32_t*>(src + 16 * s + 8 + 2 * qd)) : 0u;
-      }
-    }
-  }
   float c = a.c;
   if constexpr (Q8 && std::is_same<T, __nv_bfloat16>::value) {  // to f16, the largest to 2^10 .. 2^11
     float top = 0.f;
@@ -527,21 +528,19 @@ __global__ void __launch_bounds__((Cfg<Q8, NR>::WARPS * 32), (Cfg<Q8, NR>::PER_S
   if (S > 1) cluster_sync();  // nobody leaves while another reads its part
 }
 
-#ifndef SPLIT_COST
-#define SPLIT_COST 12
-#endif
-// Key splits (CTAs of a cluster) of `units` (sequence, kv head) pairs with up to
-// `tiles` key tiles: the fewest rounds over the SMs' CTA places times the tiles a
-// warp takes, plus what a CTA costs to start and to meet the others (about 12
-// tiles of a warp).
-int key_splits(int64_t units, int64_t tiles, int per_sm, int WARPS) {
-  const int64_t places = per_sm * (int64_t)sm_count();
+// Key splits (CTAs of a cluster) of `units` (sequence, kv head) pairs with up to `tiles`
+// key tiles: the least of rounds over the SMs' CTA places times (tiles a warp takes + 5),
+// as a CTA's start and its meeting with the others cost about five tiles.  Rounds count
+// in fractions, as lengths differ and places fill as they come free: 16 ragged sequences
+// of up to 8200 rows took 96 / 61 / 49 / 56 us with 1 / 2 / 4 / 8 CTAs each, 32 of 2049
+// rows (int8) 33 / 42 / 56 / 83.
+int key_splits(int64_t units, int64_t tiles, int per_sm, int warps) {
+  const double places = (double)per_sm * sm_count();
   int best = 1;
   double cost = 1e30;
   for (int s = 1; s <= 8; s *= 2) {
-    if (s > 1 && tiles < 2 * WARPS * s) break;
-    const double rounds = (double)((units * s + places - 1) / places);
-    const double c = rounds * ((double)tiles / (WARPS * s) + SPLIT_COST);
+    if (s > 1 && tiles < 2 * warps * s) break;
+    const double c = std::max(1.0, units * s / places) * ((double)tiles / (warps * s) + 5);
     if (c < cost - 1e-9) cost = c, best = s;
   }
   return best;
