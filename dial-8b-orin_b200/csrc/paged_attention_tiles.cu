@@ -84,6 +84,12 @@ __device__ __forceinline__ void commit(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 
+__device__ __forceinline__ bool elect() {
+  uint32_t p;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(p));
+  return p != 0;
+}
+
 // Descriptors of SWIZZLE_128B tiles whose rows are 128 bytes (8-row atoms of 1024):
 // K-major (Q, K: the row's 64 values run along K) and MN-major (V: they run along N;
 // 8-key groups 1024 bytes apart, the two 64-dim blocks HALF apart).
@@ -111,6 +117,12 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
       "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
       " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
       "r"(a), "l"(b), "r"(id), "r"(acc));
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
 }
 
 // 32 columns of the warp's 32 lanes (no wait)
@@ -160,7 +172,7 @@ __global__ void __launch_bounds__(Cfg<Q8>::THREADS, 1)
   const uint32_t base = smem_u32(smem), bars = base + L::BAR_OFF;
   float* sm_ml = reinterpret_cast<float*>(smem + L::ML_OFF);
   const uint32_t q_full = bars, o_full = bars + 8, v_fix = bars + 16, s_full = bars + 24, p_full = bars + 40;
-  const uint32_t full = bars + 56, empty = full + 8 * NS, raw_full = empty + 8 * NS, raw_empty = raw_full + 8 * 3;
+  const uint32_t full = bars + 72, empty = full + 8 * NS, raw_full = empty + 8 * NS, raw_empty = raw_full + 8 * 3;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::BAR_OFF + 248);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int* err = a.p.err;
@@ -172,7 +184,8 @@ __global__ void __launch_bounds__(Cfg<Q8>::THREADS, 1)
     mbar_init(v_fix, 1);
     for (int t = 0; t < 2; ++t) {
       mbar_init(s_full + 8 * t, 1);
-      mbar_init(p_full + 8 * t, 4);
+      mbar_init(p_full + 16 * t, 4);      // keys 0 .. 63
+      mbar_init(p_full + 16 * t + 8, 4);  // keys 64 .. 127
     }
     for (int s = 0; s < NS; ++s) {
       mbar_init(full + 8 * s, Q8 ? 4 : 1);
@@ -214,15 +227,21 @@ __global__ void __launch_bounds__(Cfg<Q8>::THREADS, 1)
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::REST_REGS));
     if (warp == 8) {
       // ------------------------------------------------ MMA issuer
-      if (lane == 0 && nj > 0) {
+      // The whole warp walks the loop and one lane issues: what is the same for all lanes stays in
+      // uniform registers, where the MMA wants its descriptors, and an MMA costs few instructions.
+      if (nj > 0) {
+        const bool lead = elect();
         bool ok = wait(q_full, 0, err);
-        auto score = [&](int j, int t) {  // S_t = Q_t K_j^T
-          const uint32_t k = base + L::RING + (uint32_t)((2 * j) % NS) * SLOT, q = base + (uint32_t)t * SLOT;
+        const uint64_t qd = desc(base, 16), kd = desc(base + L::RING, 16), vd = desc(base + L::RING, HALF);
+        auto step = [](int s) { return (uint64_t)((s >> 2) * (HALF >> 4) + 2 * (s & 3)); };  // 16 dims on
+        auto score = [&](int slot, int t) {  // S_t = Q_t K^T
+          const uint64_t q = qd + (uint64_t)(t * (SLOT >> 4)), k = kd + (uint64_t)(slot * (SLOT >> 4));
+          if (lead) {
 #pragma unroll
-          for (int s = 0; s < 8; ++s)
-            mma_ss(tmem + t * 128, desc(q + (s >> 2) * HALF, 16) + 2 * (s & 3), desc(k + (s >> 2) * HALF, 16) + 2 * (s & 3),
-                   idesc(kBf, false), s != 0);
-          commit(s_full + 8 * t);
+            for (int s = 0; s < 8; ++s) mma_ss(tmem + t * 128, q + step(s), k + step(s), idesc(kBf, false), s != 0);
+            commit(s_full + 8 * t);
+          }
+          __syncwarp();
         };
         auto full_wait = [&](int u) { return wait(full + 8 * (u % NS), (uint32_t)(u / NS) & 1u, err); };
         ok = ok && full_wait(0);
@@ -230,36 +249,45 @@ __global__ void __launch_bounds__(Cfg<Q8>::THREADS, 1)
         if (ok) {
           score(0, 0);
           if (two) score(0, 1);
-          commit(empty);
+          if (lead) commit(empty);
+          __syncwarp();
         }
+        const int ntile = two ? 2 : 1;
         for (int j = 0; j < nj && ok; ++j) {
-          const int v = 2 * j + 1;
-          for (int t = 0; t < (two ? 2 : 1) && ok; ++t) {
-            ok = wait(p_full + 8 * t, (uint32_t)j & 1u, err);
+          const int v = 2 * j + 1, vslot = v % NS, kslot = (v + 1) % NS;
+          const uint64_t vb = vd + (uint64_t)(vslot * (SLOT >> 4));
+          for (int t = 0; t < ntile && ok; ++t) {
             if (t == 0) {
-              ok = ok && full_wait(v);
+              ok = full_wait(v);
               if (!Q8 && (j0 + j + 1) * KT > ch.kv) ok = ok && wait(v_fix, 0, err);  // rows behind the cache's end
             }
-            if (!ok) break;
-            fence_after();
-            const uint64_t vd = desc(base + L::RING + (uint32_t)(v % NS) * SLOT, HALF);
 #pragma unroll
-            for (int s = 0; s < 8; ++s)
-              mma_ts(tmem + 256 + t * 128, tmem + t * 128 + 8 * s, vd + (uint64_t)(128 * s), idesc(kPBf, true), (j | s) != 0);
-            if (j + 1 < nj) {
+            for (int h = 0; h < 2; ++h) {
+              ok = ok && wait(p_full + 16 * t + 8 * h, (uint32_t)j & 1u, err);
+              fence_after();
+              if (ok && lead) {
+#pragma unroll
+                for (int s = 4 * h; s < 4 * h + 4; ++s)
+                  mma_ts(tmem + 256 + t * 128, tmem + t * 128 + 8 * s, vb + (uint64_t)(128 * s), idesc(kPBf, true), (j | s) != 0);
+              }
+              __syncwarp();
+            }
+            if (ok && j + 1 < nj) {
               if (t == 0) {
                 ok = full_wait(v + 1);
                 fence_after();
               }
-              if (ok) score(j + 1, t);
+              if (ok) score(kslot, t);
             }
           }
-          if (ok) {
-            commit(empty + 8 * (v % NS));
-            if (j + 1 < nj) commit(empty + 8 * ((v + 1) % NS));
+          if (ok && lead) {
+            commit(empty + 8 * vslot);
+            if (j + 1 < nj) commit(empty + 8 * kslot);
           }
+          __syncwarp();
         }
-        commit(o_full);
+        if (lead) commit(o_full);
+        __syncwarp();
       }
     } else if (warp == 9) {
       // ------------------------------------------------ TMA producer
@@ -418,13 +446,12 @@ __global__ void __launch_bounds__(Cfg<Q8>::THREADS, 1)
         }
         float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-        for (int e = 4; e < 128; e += 4) {
-          mx[0] = fmaxf(mx[0], s[e]);
-          mx[1] = fmaxf(mx[1], s[e + 1]);
-          mx[2] = fmaxf(mx[2], s[e + 2]);
-          mx[3] = fmaxf(mx[3], s[e + 3]);
-        }
-        float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        for (int e = 4; e < 124; e += 8)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) mx[x] = max3(mx[x], s[e + x], s[e + 4 + x]);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) mx[x] = fmaxf(mx[x], s[124 + x]);
+        float top = max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]);
         if (!Q8) top *= a.c;
         // the maximum in use moves only when the new one is far above it
         const bool move = top > m + kGrow || (m == -INFINITY && top > m);
@@ -454,37 +481,40 @@ __global__ void __launch_bounds__(Cfg<Q8>::THREADS, 1)
           }
         }
         const float sub = m == -INFINITY ? 0.f : -m;
-        float2 sum = make_float2(0.f, 0.f);
-        uint32_t pk[64];
+        // P in two halves, so that P V starts on the first
+        float2 sum = make_float2(0.f, 0.f), sum2 = sum;
 #pragma unroll
-        for (int e = 0; e < 128; e += 4) {
-          float2 x, y;
-          if constexpr (Q8) {
-            x = add2(make_float2(s[e], s[e + 1]), make_float2(sub, sub));
-            y = add2(make_float2(s[e + 2], s[e + 3]), make_float2(sub, sub));
-          } else {
-            x = fma2(make_float2(s[e], s[e + 1]), make_float2(a.c, a.c), make_float2(sub, sub));
-            y = fma2(make_float2(s[e + 2], s[e + 3]), make_float2(a.c, a.c), make_float2(sub, sub));
+        for (int h = 0; h < 2; ++h) {
+          uint32_t pk[32];
+#pragma unroll
+          for (int e = 64 * h; e < 64 * h + 64; e += 4) {
+            float2 x, y;
+            if constexpr (Q8) {
+              x = add2(make_float2(s[e], s[e + 1]), make_float2(sub, sub));
+              y = add2(make_float2(s[e + 2], s[e + 3]), make_float2(sub, sub));
+            } else {
+              x = fma2(make_float2(s[e], s[e + 1]), make_float2(a.c, a.c), make_float2(sub, sub));
+              y = fma2(make_float2(s[e + 2], s[e + 3]), make_float2(a.c, a.c), make_float2(sub, sub));
+            }
+            x.x = ex2(x.x), x.y = ex2(x.y), y.x = ex2(y.x), y.y = ex2(y.y);
+            pk[(e & 63) / 2] = pack2<PT>(x.x, x.y);
+            pk[(e & 63) / 2 + 1] = pack2<PT>(y.x, y.y);
+            if constexpr (Q8) {
+              const float4 r4 = lds16f(sc + (2 * KT + e) * 4);
+              sum = fma2(x, make_float2(r4.x, r4.y), sum);
+              sum2 = fma2(y, make_float2(r4.z, r4.w), sum2);
+            } else {
+              sum = add2(sum, x);
+              sum2 = add2(sum2, y);
+            }
           }
-          x.x = ex2(x.x), x.y = ex2(x.y), y.x = ex2(y.x), y.y = ex2(y.y);
-          pk[e / 2] = pack2<PT>(x.x, x.y);
-          pk[e / 2 + 1] = pack2<PT>(y.x, y.y);
-          if constexpr (Q8) {
-            const float4 r4 = lds16f(sc + (2 * KT + e) * 4);
-            sum = fma2(x, make_float2(r4.x, r4.y), sum);
-            sum = fma2(y, make_float2(r4.z, r4.w), sum);
-          } else {
-            sum = add2(sum, x);
-            sum = add2(sum, y);
-          }
+          tmem_st32(ts + 32 * h, pk);
+          tmem_wait_st();
+          fence_before();
+          __syncwarp();
+          if (lane == 0) arrive(p_full + 16 * t + 8 * h);
         }
-        l += sum.x + sum.y;
-        tmem_st32(ts, pk);
-        tmem_st32(ts + 32, pk + 32);
-        tmem_wait_st();
-        fence_before();
-        __syncwarp();
-        if (lane == 0) arrive(p_full + 8 * t);
+        l += (sum.x + sum.y) + (sum2.x + sum2.y);
       }
     }
     // ------------------------------------------------ epilogue

@@ -711,3 +711,29 @@ def test_paged_path_agrees_with_the_slot_cache(torch, P, D_slots=2):
     assert (k.float() - kc[0, :, :L].transpose(0, 1).float()).abs().max() <= 6 * 2.0 ** -11 * 2 * size
     # a score moves by at most 12 u |q|.|k| scale <= 12 u 128^.5 * 1.5 (unit rms rows, some larger), an output by twice that
     assert (got[0].float() - out[L - 1].float()).abs().max() <= 2 * 12 * 2.0 ** -11 * 128 ** 0.5 * 1.5 * v.float().abs().max()
+
+
+@pytest.mark.parametrize("q,kv", [([4], [300]), ([90], [300])])
+@pytest.mark.parametrize("quant", [False, True])
+def test_a_nan_score_reaches_its_rows_and_no_others(torch, P, q, kv, quant):
+    """A NaN in one value of q or of an attended key: NaN in the rows that meet it, wherever in a tile it is."""
+    s = Setup(torch, P, q, kv, "f16", quant, 64, 2)
+    x = torch.randn((s.T, 8, D), generator=gen(torch, 4), device="cuda").half()
+    good = s.cache.attention(x, s.batch)
+    for t, h in ((0, 0), (q[0] - 1, 5), (q[0] // 2, 3)):
+        keep = x[t, h, 77].clone()
+        x[t, h, 77] = math.nan
+        got = s.cache.attention(x, s.batch)
+        x[t, h, 77] = keep
+        assert torch.isnan(got[t, h]).all()
+        got[t, h] = good[t, h]
+        assert torch.equal(got, good)
+    for at in (0, 1, 2, 3, 63, 126, 131, 200):  # (all tokens see these)
+        page, row = s.host_table[0][at // 64], at % 64
+        where = s.scales[0][page, 1, row] if quant else s.pages[0][page, 1, row, 5]
+        keep = where.clone()
+        where.fill_(math.nan)
+        got = s.cache.attention(x, s.batch)
+        where.copy_(keep)
+        assert torch.isnan(got[:, 4:]).all(), at
+        assert torch.equal(got[:, :4], good[:, :4])
