@@ -20,6 +20,7 @@ The kernels are in libdial_cuda.so; there is no CPU path.
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import Optional, Sequence, Tuple
 
 from . import _torch, check, dtype_code, lib
@@ -62,28 +63,34 @@ def _tensor(t, name: str, dtype, shape: tuple, index: int):
 
 
 _fns = {}
+_cuda = None  # torch._C's current device and raw stream
+
+
+def _bind_cuda():
+    """(current device, raw current stream of a device), as bare functions where torch has
+    them: a Stream object costs 3 us a call, as much as a launch."""
+    global _cuda
+    torch = _torch()
+    dev = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+    torch.cuda.current_device()  # (initialises CUDA)
+    _cuda = dev, raw
+    return _cuda
 
 
 def _call(name: str, index: int, *args):
     """A library call on the current stream of CUDA device `index` (made current for the call)."""
-    torch = _torch()
     fn = _fns.get(name)
     if fn is None:
         fn = _fns[name] = getattr(lib(), name)
-    if index == torch.cuda.current_device():
-        status = fn(*args, _raw_stream(index))
+    dev, raw = _cuda or _bind_cuda()
+    if index == dev():
+        status = fn(*args, raw(index))
     else:
-        with torch.cuda.device(index):
-            status = fn(*args, _raw_stream(index))
+        with _torch().cuda.device(index):
+            status = fn(*args, raw(index))
     if status:
         check(status, name)
-
-
-def _raw_stream(index: int) -> int:
-    """The current stream's cudaStream_t; without the Stream object that costs 3 us a call."""
-    torch = _torch()
-    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-    return raw(index) if raw is not None else torch.cuda.current_stream(index).cuda_stream
 
 
 class PagedBatch:
@@ -282,6 +289,11 @@ def rope_tables(rows: int, theta: float, device=None):
     return cos, sin
 
 
+@functools.lru_cache(maxsize=256)
+def _verify_bytes(rows: int, vocab: int) -> int:
+    return lib().dial_verify_drafts_workspace_bytes(rows, vocab)
+
+
 def verify_drafts(logits, ids, q_start, temperature, accept_u, sample_u, draft_probs=None,
                   max_q: Optional[int] = None):
     """Verifies drafted tokens against the target's probabilities; with one row a sequence
@@ -312,10 +324,10 @@ def verify_drafts(logits, ids, q_start, temperature, accept_u, sample_u, draft_p
     if draft_probs is not None:
         _tensor(draft_probs, "draft_probs", f32, (R, V), index)
     # one allocation: tokens, counts, log-probabilities, workspace
-    need = lib().dial_verify_drafts_workspace_bytes(R, V)
+    need = _verify_bytes(R, V)
     at = (2 * R + n + 3) // 4 * 4
     buf = torch.empty(at + need // 4, dtype=i32, device=logits.device)
-    out, count, logp, _ = buf.split((R, n, R, buf.numel() - 2 * R - n))
+    out, count, logp, _ = buf.split_with_sizes((R, n, R, at + need // 4 - 2 * R - n))
     p = buf.data_ptr()
     _call("dial_verify_drafts", index, logits.data_ptr(), dtype_code(logits.dtype), ids.data_ptr(),
           draft_probs.data_ptr() if draft_probs is not None else None, q_start.data_ptr(), n,
