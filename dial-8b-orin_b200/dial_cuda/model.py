@@ -21,6 +21,7 @@ from typing import Optional
 
 from . import (BF16, F16, F32, GgufLinear, W8A16Linear, _torch, check, dtype_code, lib,
                stream_ptr)
+from .paged import PagedKVCache
 
 WFMT_W8A16, WFMT_W8A16_F16S, WFMT_Q4_0, WFMT_Q8_0 = 0, 1, 2, 8
 
@@ -252,6 +253,43 @@ class Stage:
                                          need, stream_ptr()), "dial_decoder_layers")
         return hidden
 
+    def paged_caches(self, n_pages: int, page_size: int = 64, quantized: bool = False) -> list:
+        """A `PagedKVCache` per layer of this stage, for `layers_forward_paged`."""
+        return [PagedKVCache(n_pages, self.cfg.n_kv_heads, page_size, self.dt, quantized, self.device)
+                for _ in range(self.last - self.first)]
+
+    def layers_forward_paged(self, hidden, positions, batch, caches, tables, sections=(64,), interleaved=True):
+        """This stage's layers on hidden [T, H] in place, over paged caches: the chunks of
+        `batch` (several sequences at once, prompt pieces or drafted tokens) are appended and
+        attend their sequences' pages.  positions int32 [T] or [n_axes, T] with `sections`
+        (`PagedKVCache.append`), tables: `rope_tables(rows, cfg.rope_theta)`.  Rows of hidden
+        behind the batch's last token come out unspecified."""
+        torch = _torch()
+        c, T = self.cfg, hidden.shape[0]
+        x, delta = torch.empty_like(hidden), None
+        qkv = torch.empty((T, (c.n_heads + 2 * c.n_kv_heads) * c.head_dim), dtype=self.dt, device=self.device)
+        q, attn = (torch.zeros((T, c.n_heads, c.head_dim), dtype=self.dt, device=self.device) for _ in range(2))
+        mid = torch.empty((T, c.intermediate), dtype=self.dt, device=self.device)
+
+        def norm(res, w):  # x = rms(hidden + res), hidden += res
+            check(lib().dial_rmsnorm((hidden if res is None else res).data_ptr(), None if res is None else hidden.data_ptr(),
+                                     None if res is None else hidden.data_ptr(), w.data_ptr(), x.data_ptr(),
+                                     dtype_code(self.dt), T, c.hidden, c.rms_eps, stream_ptr()), "dial_rmsnorm")
+
+        for lin, norms, cache in zip(self.layer_linears, self.layer_norms, caches):
+            norm(delta, norms["input_norm"])
+            lin["qkv"].lin.forward(x, qkv)
+            cache.append(qkv, batch, *tables, positions, q_norm=norms["q_norm"] if c.qk_norm else None,
+                         k_norm=norms["k_norm"] if c.qk_norm else None, eps=c.rms_eps, sections=sections,
+                         interleaved=interleaved, out=q)
+            cache.attention(q, batch, out=attn)
+            norm(lin["o"].lin.forward(attn.view(T, -1)), norms["post_norm"])
+            gate_up = lin["gate_up"].lin.forward(x)
+            check(lib().dial_swiglu(gate_up.data_ptr(), mid.data_ptr(), dtype_code(self.dt), T, c.intermediate,
+                                    stream_ptr()), "dial_swiglu")
+            delta = lin["down"].lin.forward(mid)
+        return hidden if delta is None else hidden.add_(delta)
+
     def head_forward(self, hidden, out_ids, row_index=None, logits=None):
         rows = out_ids.numel()
         ws, need = self.workspace(max(rows, hidden.shape[0]), 1)
@@ -341,3 +379,17 @@ class Decoder:
         st.layers_forward(hidden, positions, slots, max_len)
         st.head_forward(hidden, out_ids)
         return out_ids
+
+    def forward_paged(self, ids, positions, batch, caches, tables, sections=(64,), interleaved=True):
+        """A chunk of several sequences over paged caches (`Stage.layers_forward_paged`):
+        ids int32 [T] -> (logits [T, vocab], greedy ids [T]).  The logits of drafted tokens are
+        what `verify_drafts` takes, with the same ids and `batch.q_start`."""
+        torch = _torch()
+        st, T = self.stage, ids.numel()
+        hidden = torch.empty((T, self.cfg.hidden), device=st.device, dtype=st.dt)
+        st.embed_tokens(ids, hidden)
+        st.layers_forward_paged(hidden, positions, batch, caches, tables, sections, interleaved)
+        logits = torch.empty((T, self.cfg.vocab), device=st.device, dtype=st.dt)
+        out = torch.empty(T, device=st.device, dtype=torch.int32)
+        st.head_forward(hidden, out, logits=logits)
+        return logits, out

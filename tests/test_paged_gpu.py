@@ -737,3 +737,63 @@ def test_a_nan_score_reaches_its_rows_and_no_others(torch, P, q, kv, quant):
         where.copy_(keep)
         assert torch.isnan(got[:, 4:]).all(), at
         assert torch.equal(got[:, :4], good[:, :4])
+
+
+@pytest.mark.parametrize("act,quant", [("f16", False), ("bf16", False), ("f16", True)])
+def test_decoder_over_pages(torch, P, act, quant):
+    """Two prompts in chunks of one batch, then their greedy continuations as drafts: the logits
+    are those of the slot-cache decoder (1e-2 of the largest, the bound its own prefill and decode
+    paths are held to; int8 caches twice that), and every draft that the target repeats is accepted."""
+    from dial_cuda.model import Decoder, ModelConfig
+    cfg = ModelConfig(n_layers=2, hidden=512, intermediate=1024, n_heads=8, n_kv_heads=2, vocab=2048, act_dtype=act)
+    dec = Decoder(cfg, n_slots=2, max_seq=128)
+    g = gen(torch, 77)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    lens, n_new = (37, 20), 5
+    seqs, slot_logits = [], []
+    for b, n in enumerate(lens):
+        ids = torch.randint(0, cfg.vocab, (n,), generator=g, **i32)
+        nxt = dec.prefill(ids, slot=b)
+        toks = [ids, nxt]
+        for step in range(n_new - 1):
+            out = torch.empty(1, **i32)
+            dec.decode_step(toks[-1], torch.tensor([n + step], **i32), torch.tensor([b], **i32), n + step + 1, out)
+            toks.append(out)
+        seqs.append(torch.cat(toks))
+        hidden = torch.empty((n + n_new - 1, cfg.hidden), device="cuda", dtype=dec.stage.dt)
+        dec.stage.embed_tokens(seqs[b][:-1], hidden)
+        T = n + n_new - 1
+        dec.stage.layers_forward(hidden, torch.arange(T, **i32), torch.full((T,), b, **i32), T)
+        lg = torch.empty((T, cfg.vocab), device="cuda", dtype=dec.stage.dt)
+        dec.stage.head_forward(hidden, torch.empty(T, **i32), logits=lg)
+        slot_logits.append(lg)
+    caches = dec.stage.paged_caches(10, 16, quant)
+    tables = P.rope_tables(128, cfg.rope_theta)
+    table = torch.tensor([[4, 9, 1], [0, 7, 3]], **i32)
+
+    def chunk(spans):
+        ids = torch.cat([seqs[b][lo:hi] for b, (lo, hi) in enumerate(spans)])
+        pos = torch.cat([torch.arange(lo, hi, **i32) for lo, hi in spans])
+        start = torch.tensor([0, spans[0][1] - spans[0][0], ids.numel()], **i32)
+        batch = P.PagedBatch(table, torch.tensor([hi for _, hi in spans], **i32), start)
+        return ids, batch, dec.forward_paged(ids, pos, batch, caches, tables)[0]
+
+    bound = 1e-2 * (2 if quant else 1)
+    worst = 0.0
+    for spans in ([(0, 16), (0, 20)], [(16, 37), (20, 20)], [(37, 41), (20, 24)]):
+        ids, batch, logits = chunk(spans)
+        want = torch.cat([slot_logits[b][lo:hi] for b, (lo, hi) in enumerate(spans)])
+        worst = max(worst, float((logits.float() - want.float()).abs().max() / want.float().abs().max()))
+    assert worst <= bound, worst
+    T, u = torch.zeros(2, device="cuda"), torch.rand(ids.numel() + 2, generator=g, device="cuda")
+    out, count, _ = P.verify_drafts(logits, ids, batch.q_start, T, u[:-2].contiguous(), u[-2:].contiguous())
+    best = logits.float().argmax(-1).tolist()
+    got, s = out.tolist(), batch.q_start.tolist()
+    for b in range(2):
+        n = 0
+        while True:  # accepted while the draft is the target's best token
+            assert got[s[b] + n] == best[s[b] + n]
+            n += 1
+            if s[b] + n == s[b + 1] or int(ids[s[b] + n]) != best[s[b] + n - 1]:
+                break
+        assert int(count[b]) == n and all(x == -1 for x in got[s[b] + n:s[b + 1]])
