@@ -29,7 +29,7 @@ constexpr int kStatWarps = 4;
 constexpr int kDrawThreads = 512;
 constexpr int kWarps = kDrawThreads / 32;
 constexpr int HOLD = 5;             // vectors that a thread of the draw keeps
-constexpr int kDrawSmem = HOLD * kDrawThreads * 24 + 64 * 32 * 8;
+constexpr int kDrawSmem = HOLD * kDrawThreads * 32 + 64 * 32 * 8;
 
 struct __align__(16) SegStat {
   float m, s;                // maximum, sum of exp((x - m) / T)
@@ -56,16 +56,9 @@ struct Vec {
       if (v * N + i < total) h[i] = x[v * N + i];
     return u;
   }
-  // its values; those outside [lo, hi) and NaN as minus infinity (NAN_STAYS: but for a
-  // vector inside, whose NaN stay)
-  template <bool NAN_STAYS>
+  // its values; those outside [lo, hi) and NaN as minus infinity
   static __device__ __forceinline__ void values(uint4 u, int64_t v, int64_t lo, int64_t hi, float (&f)[N]) {
     const T* h = reinterpret_cast<const T*>(&u);
-    if (NAN_STAYS && v * N >= lo && (v + 1) * N <= hi) {
-#pragma unroll
-      for (int i = 0; i < N; ++i) f[i] = Act<T>::to_f32(h[i]);
-      return;
-    }
     const int a = (int)max(lo - v * N, (int64_t)0), b = (int)min(hi - v * N, (int64_t)N);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
@@ -128,7 +121,7 @@ __global__ void __launch_bounds__(kStatWarps * 32) verify_stats_kernel(VerifyArg
 #pragma unroll
       for (int i = 0; i < N; ++i) f[k][i] = Act<T>::to_f32(h[i]);
     } else {
-      Vec<T>::template values<false>(u[k], v0 + k * 32 + lane, lo, hi, f[k]);
+      Vec<T>::values(u[k], v0 + k * 32 + lane, lo, hi, f[k]);
     }
 #pragma unroll
     for (int i = 0; i < N; ++i) m = fmaxf(m, f[k][i]);
@@ -233,19 +226,37 @@ __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.w
 // The runs' sums meet: every warp puts its own into sum[] of every CTA of the cluster (a
 // buffer that the call before last used); afterwards every warp knows the total, the run
 // that `u` times it falls in and the sum before that run (the last run of any weight,
-// should rounding leave none).
+// should rounding leave none).  `three`: the sums are mine = sum of e, a and q, the weights
+// a - z q with z the total of e.
 template <int CL>
-__device__ __forceinline__ double meet(double* sum, int rank, double mine, double u, int& run, double& before) {
+__device__ __forceinline__ double meet(double* sum, int rank, bool three, double mine, double a, double q, double& z,
+                                       double u, int& run, double& before) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  if (lane < CL) st_cluster_f64(map_shared(sum + rank * kWarps + warp, lane), mine);
+  constexpr int ALL = CL * kWarps;
+  if (lane < CL) {
+    const uint32_t at = map_shared(sum + rank * kWarps + warp, lane);
+    st_cluster_f64(at, mine);
+    if (three) st_cluster_f64(at + ALL * 8, a), st_cluster_f64(at + 2 * ALL * 8, q);
+  }
   __syncwarp();
   cluster_sync();
-  constexpr int PER = CL * kWarps / 32;
+  constexpr int PER = ALL / 32;
   double v[PER], s = 0.0;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     v[i] = sum[lane * PER + i];
     s += v[i];
+  }
+  if (three) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    z = s;
+    s = 0.0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      v[i] = fmax(fma(-z, sum[2 * ALL + lane * PER + i], sum[ALL + lane * PER + i]), 0.0);
+      s += v[i];
+    }
   }
   double pre = s;  // inclusive prefix over the lanes
 #pragma unroll
@@ -280,11 +291,12 @@ template <typename T, int CL, int PER_SM>
 __global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(kDrawThreads, PER_SM)
     verify_draw_kernel(VerifyArgs a, const SegStat* __restrict__ stat, int nseg) {
   constexpr int N = Vec<T>::N;
-  __shared__ __align__(16) double sum[2][CL * kWarps];
+  __shared__ __align__(16) double sum[2][3 * CL * kWarps];
   extern __shared__ __align__(16) uint8_t draw_smem[];
   uint4(*held)[kDrawThreads] = reinterpret_cast<uint4(*)[kDrawThreads]>(draw_smem);  // this thread's vectors
   double(*part)[kDrawThreads] = reinterpret_cast<double(*)[kDrawThreads]>(draw_smem + HOLD * kDrawThreads * 16);  // their sums
-  double* table = reinterpret_cast<double*>(draw_smem + HOLD * kDrawThreads * 24);  // [64][32]
+  double(*partq)[kDrawThreads] = reinterpret_cast<double(*)[kDrawThreads]>(draw_smem + HOLD * kDrawThreads * 24);
+  double* table = reinterpret_cast<double*>(draw_smem + HOLD * kDrawThreads * 32);  // [64][32]
   __shared__ float row_m[kWarps], row_z[kWarps], row_x[kWarps];
   __shared__ int row_top[kWarps], row_ok[kWarps], row_draft[kWarps];
   pdl_trigger();
@@ -383,45 +395,49 @@ __global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(kDrawThreads, PER_S
   // ---- the draw from row `stop`: run w of CL * kWarps, in whole vectors
   const bool inf = m == INFINITY;  // takes everything: weights 1 at the maximum
   const Exp ex(table, inf ? 0.f : m, temp, k64);
-  const int64_t lo = stop * V, hi = lo + V, v0 = lo / N, nv = (hi + N - 1) / N - v0;
-  const int64_t per = (nv + CL * kWarps - 1) / (CL * kWarps);
-  const int64_t a0 = v0 + min(nv, (int64_t)(rank * kWarps + warp) * per), a1 = min(v0 + nv, a0 + per);
+  // (vectors counted from the row's first, which like its last may hold other rows' values)
+  const int64_t lo = stop * V, hi = lo + V, v0 = lo / N;
+  const int nv = (int)((hi + N - 1) / N - v0), per = (nv + CL * kWarps - 1) / (CL * kWarps);
+  const int a0 = min(nv, (rank * kWarps + warp) * per), a1 = min(nv, a0 + per);
+  const uint4* xv = reinterpret_cast<const uint4*>(x) + v0;
+  const float* qv = a.probs + v0 * N;
+  const bool cut = (v0 + nv) * N > total;  // the last vector passes the array's end
+  const int to_draft = draft >= 0 && draft < V ? (int)(lo + draft - v0 * N) : -1;
   double z64 = 0.0;
-  // 0: all of p; 1: p without the draft; 2: max(p - q, 0), after a pass for Z in f64
-  const int kind = !rejected ? 0 : (a.probs ? 2 : 1);
-  int mode = kind == 2 ? 0 : kind;
-  const int64_t dv = mode == 1 && draft >= 0 && draft < V ? (lo + draft) / N : -1;  // the draft's vector
-  auto weights = [&](uint4 u, int64_t v, double (&w)[N]) {
-    float f[N];
-    Vec<T>::template values<true>(u, v, lo, hi, f);
+  const double z0 = (double)Z;
+  // 0: all of p; 1: p without the draft; 3: max(p - q, 0) Z = max(e - q Z, 0) in one pass, by
+  // the sums of e and q where e > q z0, z0 being Z as the segments gave it: a value on the
+  // wrong side of that has a weight below 2^-23 of its e, and nothing else depends on z0.
+  // Where little is left (below 2^-12 of p) 2 follows: the same with Z in f64 throughout.
+  int mode = !rejected ? 0 : (a.probs ? 3 : 1);
+  auto values = [&](uint4 u, int v, float (&f)[N]) {
+    if (v == 0 || v == nv - 1) {
+      Vec<T>::values(u, v0 + v, lo, hi, f);
+    } else {
+      const T* h = reinterpret_cast<const T*>(&u);
+#pragma unroll
+      for (int i = 0; i < N; ++i) f[i] = Act<T>::to_f32(h[i]);
+    }
     if (inf) {
 #pragma unroll
       for (int i = 0; i < N; ++i) f[i] = f[i] == m ? 0.f : -INFINITY;
     }
-    if (v == dv && mode == 1) {
+    if (mode == 1 && v == to_draft / N) {
 #pragma unroll
       for (int i = 0; i < N; ++i)
-        if (v * N + i == lo + draft) f[i] = -INFINITY;
+        if (v * N + i == to_draft) f[i] = -INFINITY;
     }
+  };
+  auto draft_probs = [&](int v, float (&q)[N]) {
+    if (!cut || v < nv - 1) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) w[i] = ex(f[i]);
-    if (mode == 2) {  // max(p - q, 0) Z = max(e - q Z, 0)
-      float q[N];
-      if ((v + 1) * N <= total) {
-#pragma unroll
-        for (int i = 0; i < N; i += 4) {
-          const float4 y = __ldg(reinterpret_cast<const float4*>(a.probs + v * N + i));
-          q[i] = y.x, q[i + 1] = y.y, q[i + 2] = y.z, q[i + 3] = y.w;
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i) q[i] = v * N + i < total ? a.probs[v * N + i] : 0.f;
+      for (int i = 0; i < N; i += 4) {
+        const float4 y = __ldg(reinterpret_cast<const float4*>(qv + v * N + i));
+        q[i] = y.x, q[i + 1] = y.y, q[i + 2] = y.z, q[i + 3] = y.w;
       }
+    } else {
 #pragma unroll
-      for (int i = 0; i < N; ++i) {  // (outside the row w is nothing and stays it)
-        const double d = fma(-(double)q[i], z64, w[i]);
-        w[i] = __double2hiint(d) < 0 ? 0.0 : d;
-      }
+      for (int i = 0; i < N; ++i) q[i] = (v0 + v) * N + i < total ? qv[v * N + i] : 0.f;
     }
   };
   auto weight1 = [&](int64_t e) {  // of one element of the row
@@ -429,11 +445,13 @@ __global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(kDrawThreads, PER_S
     if (inf) f = f == m ? 0.f : -INFINITY;
     if (mode == 1 && e - lo == draft) f = -INFINITY;
     const double w = ex(f);
-    return mode == 2 ? fmax(fma(-(double)a.probs[e], z64, w), 0.0) : w;
+    if (mode < 2) return w;
+    const double q = (double)a.probs[e];
+    return mode == 3 && !(fma(-q, z0, w) > 0.0) ? 0.0 : fmax(fma(-q, z64, w), 0.0);
   };
-  if (kind == 2)  // the draft's weights of this run, wanted after the pass for Z
-    for (int64_t e = a0 * N + 32 * lane; e < min(a1 * N, total); e += 32 * 32)
-      asm volatile("prefetch.global.L2 [%0];" ::"l"(a.probs + e));
+  if (mode == 3)  // the draft's weights of this run, wanted soon
+    for (int e = a0 * N + 32 * lane; e < a1 * N && v0 * N + e < total; e += 32 * 32)
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(qv + e));
   __syncwarp();
   cluster_wait();
   const double u = (double)ut;
@@ -445,46 +463,66 @@ __global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(kDrawThreads, PER_S
   // rolled: code that runs once or twice a launch waits for its instructions.
   for (;;) {
     const bool locate = run >= 0;
-    double mine = 0.0, cum = before;
+    double mine = 0.0, mina = 0.0, minq = 0.0, cum = before;
     bool found = false;
 #pragma unroll 1
-    for (int64_t c0 = a0; c0 < a1 && !found; c0 += 32 * HOLD) {
+    for (int c0 = a0; c0 < a1 && !found; c0 += 32 * HOLD) {
       if (!locate || !single) {
         if (!single || !loaded) {  // all in flight at once; each thread reads back its own
 #pragma unroll
           for (int k = 0; k < HOLD; ++k) {
-            const int64_t v = c0 + 32 * k + lane;
-            if (v < a1 && (v + 1) * N <= total)
+            const int v = c0 + 32 * k + lane;
+            if (v < a1 && !(cut && v == nv - 1))
               asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(&held[k][threadIdx.x])),
-                           "l"(reinterpret_cast<const uint4*>(x) + v)
+                           "l"(xv + v)
                            : "memory");
             else if (v < a1)
-              held[k][threadIdx.x] = Vec<T>::load(x, v, total);
+              held[k][threadIdx.x] = Vec<T>::load(x, v0 + v, total);
           }
           asm volatile("cp.async.wait_all;" ::: "memory");
           loaded = true;
         }
 #pragma unroll 1
         for (int k = 0; k < HOLD; ++k) {
-          const int64_t v = c0 + 32 * k + lane;
-          double s = 0.0;
+          const int v = c0 + 32 * k + lane;
+          double s = 0.0, sa = 0.0, sq = 0.0;
           if (v < a1) {
-            double w[N];
-            weights(held[k][threadIdx.x], v, w);
+            float f[N];
+            values(held[k][threadIdx.x], v, f);
+            if (mode >= 2) {  // (outside the row e is nothing, and not above q z0 unless q is 0)
+              float q[N];
+              draft_probs(v, q);
+              const double z = mode == 3 ? z0 : z64;
 #pragma unroll
-            for (int i = 0; i < N; i += 2) s += w[i] + w[i + 1];
+              for (int i = 0; i < N; ++i) {
+                const double w = ex(f[i]), qd = (double)q[i], d = fma(-qd, z, w);
+                const bool over = __double2hiint(d) >= 0;
+                s += mode == 3 ? w : (over ? d : 0.0);
+                sa += over ? w : 0.0;
+                sq += over ? qd : 0.0;
+              }
+            } else {
+              double s2 = 0.0;
+#pragma unroll
+              for (int i = 0; i < N; i += 2) s += ex(f[i]), s2 += ex(f[i + 1]);
+              s += s2;
+            }
           }
-          part[k][threadIdx.x] = s;
+          part[k][threadIdx.x] = mode == 3 ? sa : s;
+          partq[k][threadIdx.x] = sq;
           mine += s;
+          mina += sa;
+          minq += sq;
         }
       }
       if (!locate) continue;
       // the vector in which the cumulative sum passes `at`, or the last of any weight
-      int64_t vec = -1;
+      int vec = -1;
       double start = 0.0;
 #pragma unroll 1
       for (int k = 0; k < HOLD && !found; ++k) {
-        const double s = part[k][threadIdx.x];
+        double s = part[k][threadIdx.x];
+        if (mode == 3) s = fmax(fma(-z64, partq[k][threadIdx.x], s), 0.0);
         double pre = s;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -502,7 +540,7 @@ __global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(kDrawThreads, PER_S
         cum += __shfl_sync(0xffffffffu, pre, 31);
       }
       if (vec >= 0) {  // its element, a lane each
-        const int64_t e = vec * N + lane;
+        const int64_t e = (v0 + vec) * N + lane;
         const double w = lane < N && e >= lo && e < hi ? weight1(e) : 0.0;
         double pre = w;
 #pragma unroll
@@ -512,19 +550,21 @@ __global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(kDrawThreads, PER_S
         }
         const unsigned some = __ballot_sync(0xffffffffu, w > kNone && start + pre > at);
         const unsigned any = __ballot_sync(0xffffffffu, w > kNone);
-        token = (int)(vec * N + (some ? __ffs(some) - 1 : 31 - __clz(any)) - lo);
+        token = (int)((v0 + vec) * N + (some ? __ffs(some) - 1 : 31 - __clz(any)) - lo);
       }
     }
     if (locate) break;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+    for (int o = 16; o > 0; o >>= 1) {
+      mine += __shfl_xor_sync(0xffffffffu, mine, o);
+      if (mode == 3) mina += __shfl_xor_sync(0xffffffffu, mina, o), minq += __shfl_xor_sync(0xffffffffu, minq, o);
+    }
     int r;
-    all = meet<CL>(sum[buf], rank, mine, u, r, before);
+    all = meet<CL>(sum[buf], rank, mode == 3, mine, mina, minq, z64, u, r, before);
     buf ^= 1;
-    if (kind == 2 && z64 == 0.0) {
-      z64 = all;
+    if (mode == 3 && !(all > z64 * 0x1p-12)) {
       mode = 2;
-    } else if (mode && !(all > kNone)) {
+    } else if (mode && mode != 3 && !(all > kNone)) {
       mode = 0;  // nothing left of it: from p
     } else {
       if (r != rank * kWarps + warp) break;
