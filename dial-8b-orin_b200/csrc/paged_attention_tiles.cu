@@ -178,6 +178,23 @@ __global__ void __launch_bounds__(Cfg<Q8>::THREADS, 1)
   int* err = a.p.err;
 
   pdl_trigger();
+  pdl_wait();
+
+  // ---- this CTA's rows and keys: heavy tiles first
+  const int S = (int)cluster_size(), rank = (int)cluster_rank();
+  const int per = a.p.n_seqs * a.p.hkv, unit = blockIdx.x / S;
+  const int tiles = gridDim.x / S / per;
+  const int qt = tiles - 1 - unit / per, b = unit % per / a.p.hkv, g = unit % a.p.hkv;
+  const Chunk ch = chunk_of(a.p, b, threadIdx.x == 0);
+  const int i0 = qt * 2 * a.tpt;                       // first token (of the chunk) of this CTA
+  const int ntok = min(ch.n - i0, 2 * a.tpt);          // its tokens; <= 0: nothing to do
+  if (S == 1 && ntok <= 0) return;                     // a shorter chunk than the longest
+  const bool two = ntok > a.tpt;
+  const int before = ch.kv - ch.n;                     // token i sees keys 0 .. before + i
+  const int len = ntok > 0 ? max(0, before + i0 + ntok) : 0;
+  const int nkt = (len + KT - 1) / KT;
+  const int j0 = (int)((int64_t)nkt * rank / S), nj = (int)((int64_t)nkt * (rank + 1) / S) - j0;
+
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
     mbar_init(o_full, 1);
@@ -207,21 +224,6 @@ __global__ void __launch_bounds__(Cfg<Q8>::THREADS, 1)
   __syncthreads();
   fence_after();
   const uint32_t tmem = *tmem_slot;
-  pdl_wait();
-
-  // ---- this CTA's rows and keys: heavy tiles first
-  const int S = (int)cluster_size(), rank = (int)cluster_rank();
-  const int per = a.p.n_seqs * a.p.hkv, unit = blockIdx.x / S;
-  const int tiles = gridDim.x / S / per;
-  const int qt = tiles - 1 - unit / per, b = unit % per / a.p.hkv, g = unit % a.p.hkv;
-  const Chunk ch = chunk_of(a.p, b, threadIdx.x == 0);
-  const int i0 = qt * 2 * a.tpt;                       // first token (of the chunk) of this CTA
-  const int ntok = min(ch.n - i0, 2 * a.tpt);          // its tokens; <= 0: nothing to do
-  const bool two = ntok > a.tpt;
-  const int before = ch.kv - ch.n;                     // token i sees keys 0 .. before + i
-  const int len = ntok > 0 ? max(0, before + i0 + ntok) : 0;
-  const int nkt = (len + KT - 1) / KT;
-  const int j0 = (int)((int64_t)nkt * rank / S), nj = (int)((int64_t)nkt * (rank + 1) / S) - j0;
 
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::REST_REGS));
