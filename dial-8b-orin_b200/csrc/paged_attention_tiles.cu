@@ -159,6 +159,34 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
       : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return d;
 }
+// The t-th query tile (of two times 128 rows) of the batch: sequence by sequence, a chunk's
+// last tile, which sees the most keys, first.  False behind the last.  By a whole warp, a
+// sequence per lane.
+__device__ __forceinline__ bool tile_of(const Args& a, int t, int& qt, int& b) {
+  const int lane = threadIdx.x & 31, rows = 2 * a.tpt;
+  const bool report = blockIdx.x == 0 && threadIdx.x < 32;
+  bool found = false;
+  for (int i = 0; i < a.p.n_seqs && (!found || report); i += 32) {
+    int n = 0;
+    if (i + lane < a.p.n_seqs) n = (chunk_of(a.p, i + lane, report).n + rows - 1) / rows;
+    int sum = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += y;
+    }
+    const unsigned past = __ballot_sync(0xffffffffu, sum > t);
+    if (past && !found) {
+      const int l = __ffs(past) - 1;
+      b = i + l;
+      qt = __shfl_sync(0xffffffffu, sum, l) - 1 - t;
+      found = true;
+    }
+    t -= __shfl_sync(0xffffffffu, sum, 31);
+  }
+  return found;
+}
+
 template <typename T, bool Q8>
 __global__ void __launch_bounds__(Cfg<Q8>::THREADS, 1)
     paged_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
@@ -180,18 +208,17 @@ __global__ void __launch_bounds__(Cfg<Q8>::THREADS, 1)
   pdl_trigger();
   pdl_wait();
 
-  // ---- this CTA's rows and keys: heavy tiles first
+  // ---- this CTA's rows and keys
   const int S = (int)cluster_size(), rank = (int)cluster_rank();
-  const int per = a.p.n_seqs * a.p.hkv, unit = blockIdx.x / S;
-  const int tiles = gridDim.x / S / per;
-  const int qt = tiles - 1 - unit / per, b = unit % per / a.p.hkv, g = unit % a.p.hkv;
-  const Chunk ch = chunk_of(a.p, b, threadIdx.x == 0);
+  const int unit = blockIdx.x / S, g = unit % a.p.hkv;
+  int qt, b;                                           // tile of its chunk, sequence
+  if (!tile_of(a, unit / a.p.hkv, qt, b)) return;      // the grid is an upper bound
+  const Chunk ch = chunk_of(a.p, b, false);
   const int i0 = qt * 2 * a.tpt;                       // first token (of the chunk) of this CTA
-  const int ntok = min(ch.n - i0, 2 * a.tpt);          // its tokens; <= 0: nothing to do
-  if (S == 1 && ntok <= 0) return;                     // a shorter chunk than the longest
+  const int ntok = min(ch.n - i0, 2 * a.tpt);          // its tokens
   const bool two = ntok > a.tpt;
   const int before = ch.kv - ch.n;                     // token i sees keys 0 .. before + i
-  const int len = ntok > 0 ? max(0, before + i0 + ntok) : 0;
+  const int len = max(0, before + i0 + ntok);
   const int nkt = (len + KT - 1) / KT;
   const int j0 = (int)((int64_t)nkt * rank / S), nj = (int)((int64_t)nkt * (rank + 1) / S) - j0;
 
@@ -662,7 +689,10 @@ dial_status launch(const void* q, const PagedView& p, void* out, int hq, int64_t
   if (s != DIAL_OK) return s;
   cudaError_t e = ensure_smem<kern>(smem);
   if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(paged_attention_kernel)");
-  const int64_t tiles = (p.max_q + 2 * tpt - 1) / (2 * tpt), units = tiles * p.n_seqs * p.hkv;
+  // no more tiles than the longest chunk's for every sequence, nor than the tokens fill plus
+  // a broken one each
+  const int64_t tiles = std::min((int64_t)p.n_seqs * ((p.max_q + 2 * tpt - 1) / (2 * tpt)), p.tokens / (2 * tpt) + p.n_seqs);
+  const int64_t units = tiles * p.hkv;
   const int S = key_splits(units, (max_kv + KT - 1) / KT);
   if (units * S >= (1ll << 31)) return fail(DIAL_ERR_SHAPE, "too many query tiles (%lld)", (long long)units);
   cudaLaunchConfig_t cfg = {};
