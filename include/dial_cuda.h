@@ -438,7 +438,8 @@ typedef struct dial_paged_kv {
  * memory and are checked there: a page id outside [0, n_pages), q_start that falls
  * or passes `tokens`, a chunk longer than max_q or kv_len beyond max_pages pages
  * sets the device error flag (DIAL_ERR_INVALID_ARG) and touches no memory outside
- * the given arrays; that sequence's results are then unspecified. */
+ * the given arrays; that sequence's results are then unspecified (and other calls
+ * may give up early until dial_device_error(1) clears the flag). */
 typedef struct dial_paged_batch {
   const int32_t* block_table; /* [n_seqs, max_pages] */
   const int32_t* kv_len;      /* [n_seqs] */
@@ -499,8 +500,9 @@ DIAL_API dial_status dial_paged_attention(const void* q, const dial_paged_kv* kv
  * In order, a draft x is accepted if accept_u[r] * q(x) < p(x) (u in [0, 1)); at the
  * first that is not, a token is drawn from max(p - q, 0) (p if nothing is left of
  * it), and behind the last draft one from p: the first index whose cumulative
- * weight exceeds sample_u[b] times the total.  temperature 0: drafts must equal the
- * first index of the largest logit, which also is the token drawn.
+ * weight exceeds sample_u[b] times the total.  temperature 0 (or below, or NaN):
+ * drafts must equal the first index of the largest logit, which also is the token
+ * drawn.
  * out_ids[r] = the token that follows row r's prefix (an accepted draft, then the
  * drawn token), -1 behind it; n_out[b] = the number of tokens (accepted + 1; 0 for
  * a sequence without rows); logprobs[r] (optional) = log p of it (temperature 1 for
@@ -508,7 +510,8 @@ DIAL_API dial_status dial_paged_attention(const void* q, const dial_paged_kv* kv
  * without any probability token 0 is drawn, with logprob -inf; an infinite logit
  * takes all of it.  A draft outside the vocabulary is rejected.  max_q: no sequence
  * has more rows (a longer one, or a q_start that falls or passes `rows`, sets the
- * device error flag).  `workspace`: dial_verify_drafts_workspace_bytes(rows, vocab)
+ * device error flag).  logits and draft_probs are 16-byte aligned; rows of any
+ * length.  `workspace`: dial_verify_drafts_workspace_bytes(rows, vocab)
  * bytes, 16-byte aligned, any contents; calls sharing it must not overlap. */
 DIAL_API size_t dial_verify_drafts_workspace_bytes(int64_t rows, int64_t vocab);
 DIAL_API dial_status dial_verify_drafts(const void* logits, dial_dtype dt, const int32_t* ids,
