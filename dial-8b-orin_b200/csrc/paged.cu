@@ -1,5 +1,6 @@
 // Paged KV caches: the post-QKV step that writes pages, and reading them back.
 #include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
 #include "paged.cuh"
@@ -10,30 +11,30 @@ namespace {
 
 constexpr int D = 128;
 
-// Four values as two pairs.
+// Eight values as four pairs.
 template <typename T>
-__device__ __forceinline__ void unpack4(uint2 u, float2 (&v)[2]);
-template <>
-__device__ __forceinline__ void unpack4<__half>(uint2 u, float2 (&v)[2]) {
-  v[0] = __half22float2(*reinterpret_cast<const __half2*>(&u.x));
-  v[1] = __half22float2(*reinterpret_cast<const __half2*>(&u.y));
-}
-template <>
-__device__ __forceinline__ void unpack4<__nv_bfloat16>(uint2 u, float2 (&v)[2]) {
-  v[0] = make_float2(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xFFFF0000u));
-  v[1] = make_float2(__uint_as_float(u.y << 16), __uint_as_float(u.y & 0xFFFF0000u));
+__device__ __forceinline__ void unpack8(uint4 u, float2 (&v)[4]) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (std::is_same<T, __half>::value) v[i] = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+    else v[i] = make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xFFFF0000u));
+  }
 }
 template <typename T>
-__device__ __forceinline__ uint2 pack4(const float2 (&v)[2]);
-template <>
-__device__ __forceinline__ uint2 pack4<__half>(const float2 (&v)[2]) {
-  const __half2 a = __float22half2_rn(v[0]), b = __float22half2_rn(v[1]);
-  return make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
-}
-template <>
-__device__ __forceinline__ uint2 pack4<__nv_bfloat16>(const float2 (&v)[2]) {
-  const __nv_bfloat162 a = __float22bfloat162_rn(v[0]), b = __float22bfloat162_rn(v[1]);
-  return make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+__device__ __forceinline__ uint4 pack8(const float2 (&v)[4]) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (std::is_same<T, __half>::value) {
+      const __half2 h = __float22half2_rn(v[i]);
+      w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    } else {
+      const __nv_bfloat162 h = __float22bfloat162_rn(v[i]);
+      w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
 }
 __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
   float2 d;
@@ -58,11 +59,13 @@ __device__ __forceinline__ uint32_t code(float x, float inv) {
 }
 
 // ------------------------------------------------------------------ append
-// A half-warp per head: lane j of 16 holds elements 4j .. 4j+3 and 64+4j .. 64+4j+3, so
-// the pairs (i, i + 64) stay in the lane.  `wpt` warps share a token: each looks up the page
-// row and the token's cosines, then walks heads, the next one's values on their way while
-// it works on one.  Few tokens: a head each; many: as few warps a token as fill the SMs, as
-// the look-ups cost about what a head does.  Bound by the bytes of qkv, q and the cache rows.
+// Eight lanes per head: lane j holds elements 8j .. 8j+7 and 64+8j .. 64+8j+7, so the
+// pairs (i, i + 64) stay in the lane, and four heads share a warp's look-ups, shuffles and
+// reciprocal root.  `wpt` warps share a token: each looks up the page row and the token's
+// cosines, then walks heads, the next ones' values on their way while it works on four.
+// Few tokens: a head per eight lanes once; many: as few warps a token as fill the SMs, as
+// the look-ups cost about what four heads do.  Bound by instruction issue (about 60 a head
+// and warp); the bytes of qkv, q and the cache rows need half its time.
 // The mean square is summed in f64 (its squares are exact there) and 1/sqrt refined by one
 // Newton step in f64, so that the f32 factor -- and with it every int8 code -- does not
 // depend on the order of a sum; each later product is rounded to f32 on its own for the
@@ -75,24 +78,24 @@ __global__ void __launch_bounds__(256)
   if (blockIdx.x == 0)
     for (int b = threadIdx.x; b < p.n_seqs; b += blockDim.x) chunk_of(p, b, true);
   if (t >= p.tokens) return;
-  const int heads = hq + 2 * p.hkv, step = 2 * wpt;
-  const int j = threadIdx.x & 15;
-  const unsigned half = 0xFFFFu << (threadIdx.x & 16);
-  int h = (int)(w - t * wpt) * 2 + ((threadIdx.x >> 4) & 1);
-  const T* tok = qkv + (t * heads + h) * D;  // of head h
-  uint2 na = make_uint2(0, 0), nz = na;
+  const int heads = hq + 2 * p.hkv, step = 4 * wpt;
+  const int j = threadIdx.x & 7;
+  const unsigned part = 0xFFu << (threadIdx.x & 24);
+  int h = (int)(w - t * wpt) * 4 + ((threadIdx.x >> 3) & 3);
+  const T* tok = qkv + (t * heads + h) * D + 8 * j;  // this lane's first values of head h
+  uint4 na = make_uint4(0, 0, 0, 0), nz = na;
   if (h < heads) {
-    na = __ldg(reinterpret_cast<const uint2*>(tok) + j);
-    nz = __ldg(reinterpret_cast<const uint2*>(tok + 64) + j);
+    na = __ldg(reinterpret_cast<const uint4*>(tok));
+    nz = __ldg(reinterpret_cast<const uint4*>(tok + 64));
   }
   const int b = seq_of_token(p, t);
   if (b >= p.n_seqs) return;  // behind the last sequence
   const Chunk c = chunk_of(p, b, false);
   if (t < c.q0 || t >= c.q0 + c.n) return;
   // the token's turns
-  float cs[4], sn[4];
+  float2 cs[4], sn[4];
   {
-    const uint32_t axes = r.axis[j >> 2] >> (8 * (j & 3));
+    const uint32_t axes = r.axis[j >> 1] >> (16 * (j & 1));
     int row[4] = {0, 0, 0, 0};
 #pragma unroll
     for (int x = 0; x < 4; ++x)
@@ -105,16 +108,22 @@ __global__ void __launch_bounds__(256)
         row[x] = v;
       }
     if (r.n_axes == 1) {
-      const float4 x = __ldg(reinterpret_cast<const float4*>(r.cos_t + (int64_t)row[0] * (D / 2)) + j);
-      const float4 y = __ldg(reinterpret_cast<const float4*>(r.sin_t + (int64_t)row[0] * (D / 2)) + j);
-      cs[0] = x.x, cs[1] = x.y, cs[2] = x.z, cs[3] = x.w;
-      sn[0] = y.x, sn[1] = y.y, sn[2] = y.z, sn[3] = y.w;
+      const float4* x = reinterpret_cast<const float4*>(r.cos_t + (int64_t)row[0] * (D / 2) + 8 * j);
+      const float4* y = reinterpret_cast<const float4*>(r.sin_t + (int64_t)row[0] * (D / 2) + 8 * j);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float4 u = __ldg(x + i), v = __ldg(y + i);
+        cs[2 * i] = make_float2(u.x, u.y), cs[2 * i + 1] = make_float2(u.z, u.w);
+        sn[2 * i] = make_float2(v.x, v.y), sn[2 * i + 1] = make_float2(v.z, v.w);
+      }
     } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < 8; ++i) {
         const int ax = (axes >> (2 * i)) & 3;
-        const int64_t at = (int64_t)(ax == 0 ? row[0] : ax == 1 ? row[1] : ax == 2 ? row[2] : row[3]) * (D / 2) + 4 * j + i;
-        cs[i] = __ldg(r.cos_t + at), sn[i] = __ldg(r.sin_t + at);
+        const int64_t at = (int64_t)(ax == 0 ? row[0] : ax == 1 ? row[1] : ax == 2 ? row[2] : row[3]) * (D / 2) + 8 * j + i;
+        const float u = __ldg(r.cos_t + at), v = __ldg(r.sin_t + at);
+        if (i & 1) cs[i / 2].y = u, sn[i / 2].y = v;
+        else cs[i / 2].x = u, sn[i / 2].x = v;
       }
     }
   }
@@ -129,34 +138,36 @@ __global__ void __launch_bounds__(256)
       row0 = (((int64_t)page * p.hkv) << p.log2_page) + (at & ((1 << p.log2_page) - 1));
     }
   }
-  const float2 cp[2] = {{cs[0], cs[1]}, {cs[2], cs[3]}}, sp[2] = {{sn[0], sn[1]}, {sn[2], sn[3]}};
-  float2 wa[2] = {}, wz[2] = {};  // norm weights of the heads at hand: q's, then k's
+  float2 wa[4] = {}, wz[4] = {};  // norm weights of the heads at hand: q's, then k's
   int kind = 0;
-  T* qdst = q_out + t * hq * D + h * D + 4 * j;
+  T* qdst = q_out + (t * hq + h) * D + 8 * j;
   for (; h < heads; h += step, tok += step * D, qdst += step * D) {
-    float2 a[2], z[2];
-    unpack4<T>(na, a);
-    unpack4<T>(nz, z);
+    float2 a[4], z[4];
+    unpack8<T>(na, a);
+    unpack8<T>(nz, z);
     if (h + step < heads) {
-      na = __ldg(reinterpret_cast<const uint2*>(tok + step * D) + j);
-      nz = __ldg(reinterpret_cast<const uint2*>(tok + step * D + 64) + j);
+      na = __ldg(reinterpret_cast<const uint4*>(tok + step * D));
+      nz = __ldg(reinterpret_cast<const uint4*>(tok + step * D + 64));
     }
     if (h < hq + p.hkv) {
       if (r.qn) {
         const int now = h < hq ? 1 : 2;
         if (now != kind) {
-          const T* w = static_cast<const T*>(h < hq ? r.qn : r.kn);
-          unpack4<T>(__ldg(reinterpret_cast<const uint2*>(w) + j), wa);
-          unpack4<T>(__ldg(reinterpret_cast<const uint2*>(w + 64) + j), wz);
+          const T* wt = static_cast<const T*>(h < hq ? r.qn : r.kn) + 8 * j;
+          unpack8<T>(__ldg(reinterpret_cast<const uint4*>(wt)), wa);
+          unpack8<T>(__ldg(reinterpret_cast<const uint4*>(wt + 64)), wz);
           kind = now;
         }
-        const double d[8] = {a[0].x, a[0].y, a[1].x, a[1].y, z[0].x, z[0].y, z[1].x, z[1].y};
-        double ss = d[0] * d[0], s2 = d[4] * d[4];
+        double ss = 0.0, s2 = 0.0;
 #pragma unroll
-        for (int i = 1; i < 4; ++i) ss = fma(d[i], d[i], ss), s2 = fma(d[4 + i], d[4 + i], s2);
+        for (int i = 0; i < 4; ++i) {
+          const double x = a[i].x, y = a[i].y, u = z[i].x, v = z[i].y;
+          ss = fma(x, x, ss), s2 = fma(u, u, s2);
+          ss = fma(y, y, ss), s2 = fma(v, v, s2);
+        }
         ss += s2;
 #pragma unroll
-        for (int o = 8; o > 0; o >>= 1) ss += __shfl_xor_sync(half, ss, o);
+        for (int o = 4; o > 0; o >>= 1) ss += __shfl_xor_sync(part, ss, o);
         const double m = fma(ss, 1.0 / D, (double)r.eps);
         const float mf = (float)m;
         double y;
@@ -169,22 +180,22 @@ __global__ void __launch_bounds__(256)
         const float inv = (float)y;
         const float2 iv = make_float2(inv, inv);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < 4; ++i) {
           a[i] = mul2(mul2(a[i], iv), wa[i]);
           z[i] = mul2(mul2(z[i], iv), wz[i]);
         }
       }
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
+      for (int i = 0; i < 4; ++i) {
         const float2 x = a[i], y = z[i];
-        a[i].x = __fsub_rn(__fmul_rn(x.x, cp[i].x), __fmul_rn(y.x, sp[i].x));
-        a[i].y = __fsub_rn(__fmul_rn(x.y, cp[i].y), __fmul_rn(y.y, sp[i].y));
-        z[i].x = __fadd_rn(__fmul_rn(x.x, sp[i].x), __fmul_rn(y.x, cp[i].x));
-        z[i].y = __fadd_rn(__fmul_rn(x.y, sp[i].y), __fmul_rn(y.y, cp[i].y));
+        a[i].x = __fsub_rn(__fmul_rn(x.x, cs[i].x), __fmul_rn(y.x, sn[i].x));
+        a[i].y = __fsub_rn(__fmul_rn(x.y, cs[i].y), __fmul_rn(y.y, sn[i].y));
+        z[i].x = __fadd_rn(__fmul_rn(x.x, sn[i].x), __fmul_rn(y.x, cs[i].x));
+        z[i].y = __fadd_rn(__fmul_rn(x.y, sn[i].y), __fmul_rn(y.y, cs[i].y));
       }
       if (h < hq) {
-        *reinterpret_cast<uint2*>(qdst) = pack4<T>(a);
-        *reinterpret_cast<uint2*>(qdst + 64) = pack4<T>(z);
+        *reinterpret_cast<uint4*>(qdst) = pack8<T>(a);
+        *reinterpret_cast<uint4*>(qdst + 64) = pack8<T>(z);
         continue;
       }
     }
@@ -195,34 +206,36 @@ __global__ void __launch_bounds__(256)
       float amax = 0.f;
       bool odd = false;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
+      for (int i = 0; i < 4; ++i) {
         const float v[4] = {a[i].x, a[i].y, z[i].x, z[i].y};
 #pragma unroll
         for (int x = 0; x < 4; ++x) amax = fmaxf(amax, fabsf(v[x])), odd |= !(fabsf(v[x]) < INFINITY);
       }
 #pragma unroll
-      for (int o = 8; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(half, amax, o));
-      odd = __any_sync(half, odd);
+      for (int o = 4; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(part, amax, o));
+      odd = __any_sync(part, odd);
       float s, inv;
       row_scale(amax, s, inv);
-      uint32_t lo = 0, hi = 0;
+      uint2 lo = make_uint2(0, 0), hi = lo;
       if (odd) {
         s = __int_as_float(0x7fc00000);  // a row with a NaN or an infinity is kept as NaN
       } else {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          lo |= (code(a[i].x, inv) | code(a[i].y, inv) << 8) << (16 * i);
-          hi |= (code(z[i].x, inv) | code(z[i].y, inv) << 8) << (16 * i);
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t x = (code(a[i].x, inv) | code(a[i].y, inv) << 8) << (16 * (i & 1));
+          const uint32_t y = (code(z[i].x, inv) | code(z[i].y, inv) << 8) << (16 * (i & 1));
+          if (i < 2) lo.x |= x, hi.x |= y;
+          else lo.y |= x, hi.y |= y;
         }
       }
-      uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<int8_t*>(const_cast<void*>(is_k ? p.k : p.v)) + row * D);
-      dst[j] = lo;
-      dst[16 + j] = hi;
+      int8_t* dst = static_cast<int8_t*>(const_cast<void*>(is_k ? p.k : p.v)) + row * D + 8 * j;
+      *reinterpret_cast<uint2*>(dst) = lo;
+      *reinterpret_cast<uint2*>(dst + 64) = hi;
       if (j == 0) const_cast<float*>(is_k ? p.ks : p.vs)[row] = s;
     } else {
-      T* dst = static_cast<T*>(const_cast<void*>(is_k ? p.k : p.v)) + row * D;
-      reinterpret_cast<uint2*>(dst)[j] = pack4<T>(a);
-      reinterpret_cast<uint2*>(dst + 64)[j] = pack4<T>(z);
+      T* dst = static_cast<T*>(const_cast<void*>(is_k ? p.k : p.v)) + row * D + 8 * j;
+      *reinterpret_cast<uint4*>(dst) = pack8<T>(a);
+      *reinterpret_cast<uint4*>(dst + 64) = pack8<T>(z);
     }
   }
 }
@@ -289,8 +302,8 @@ __global__ void __launch_bounds__(256)
 template <typename T>
 static dial_status append_t(const void* qkv, const RopeArgs& r, const PagedView& p, int format, void* q_out,
                             int hq, cudaStream_t st) {
-  const int most = (hq + 2 * p.hkv + 1) / 2;  // a half-warp per head
-  const int wpt = (int)std::min<int64_t>(most, std::max<int64_t>(2, 32 * (int64_t)sm_count() / p.tokens));
+  const int most = (hq + 2 * p.hkv + 3) / 4;  // eight lanes per head
+  const int wpt = (int)std::min<int64_t>(most, std::max<int64_t>(1, 16 * (int64_t)sm_count() / p.tokens));
   const int64_t blocks = (p.tokens * wpt + 7) / 8;
   if (blocks >= (1ll << 31)) return fail(DIAL_ERR_SHAPE, "too many tokens (%lld)", (long long)p.tokens);
   const dim3 grid((unsigned)blocks);
