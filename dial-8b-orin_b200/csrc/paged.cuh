@@ -59,19 +59,24 @@ __device__ __forceinline__ int64_t pool_row(const PagedView& p, int b, int g, in
   return ((page_of(p, b, r >> p.log2_page) * p.hkv + g) << p.log2_page) + (r & ((1 << p.log2_page) - 1));
 }
 
-// Which sequence token t belongs to, by a whole warp (all lanes pass the same
-// t): the number of q_start[1..n_seqs] at or below t, 32 of them per round of
-// loads.  n_seqs if t lies behind the last.
-__device__ __forceinline__ int seq_of_token(const PagedView& p, int64_t t) {
+// Which sequence token t belongs to, by a whole warp (all lanes pass the same t): the
+// number of q_start[1..n_seqs] at or below t, by 32-way steps (two rounds of loads for up to
+// 1024 sequences; 32 per round took 12.6 us instead of 7.3 to append one token to each of
+// 1024 sequences).  n_seqs if t lies behind the last; in any case within [0, n_seqs].
+__device__ __forceinline__ int seq_of_token(const int32_t* __restrict__ q_start, int n_seqs, int64_t t) {
   const int lane = threadIdx.x & 31;
-  int b = 0;
-  for (int i = 0; i < p.n_seqs; i += 32) {
-    const bool past = i + lane < p.n_seqs && __ldg(p.q_start + i + lane + 1) <= t;
+  int lo = 0, n = n_seqs;
+  while (n > 0) {
+    const int stride = (n + 31) / 32, at = (lane + 1) * stride;
+    // a lane's probe is the end of its run of `stride` sequences (the last one may be shorter)
+    const bool past = lane * stride < n && __ldg(q_start + lo + min(at, n)) <= t;
     const int c = __popc(__ballot_sync(0xffffffffu, past));
-    b += c;
-    if (c < 32) break;
+    if (stride == 1) return lo + c;
+    if (c * stride >= n) return lo + n;
+    lo += c * stride;
+    n = min(stride, n - c * stride);
   }
-  return b;
+  return lo;
 }
 
 struct RopeArgs {

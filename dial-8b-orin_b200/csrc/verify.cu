@@ -103,13 +103,7 @@ __global__ void __launch_bounds__(kStatWarps * 32) verify_stats_kernel(VerifyArg
   uint4 u[PER];
 #pragma unroll
   for (int k = 0; k < PER; ++k) u[k] = Vec<T>::load(x, v0 + k * 32 + lane, total);
-  int b = 0;  // the row's sequence
-  for (int i = 0; i < a.n_seqs; i += 32) {
-    const bool past = i + lane < a.n_seqs && __ldg(a.q_start + i + lane + 1) <= row;
-    const int c = __popc(__ballot_sync(0xffffffffu, past));
-    b += c;
-    if (c < 32) break;
-  }
+  const int b = seq_of_token(a.q_start, a.n_seqs, row);
   if (b >= a.n_seqs) return;
   const float temp = a.temperature[b], it = log2e_over(temp);
   float f[PER][N], m = -INFINITY;

@@ -134,7 +134,8 @@ def axis_of(axes, interleaved):
 
 
 @pytest.mark.parametrize("q,kv,pad", [([1], [1], 0), ([1], [2049], 3), ([7, 0, 33, 1], [7, 5, 49, 16], 2),
-                                      ([20, 40], [64, 31], 0), ([1] * 70, list(range(1, 71)), 1)])
+                                      ([20, 40], [64, 31], 0), ([1] * 70, list(range(1, 71)), 1),
+                                      ([(2, 0, 1)[b % 3] for b in range(1100)], [3 + b % 40 for b in range(1100)], 2)])
 @pytest.mark.parametrize("dtype,quant,page,hq,hkv,axes,interleaved,norm", [
     ("f16", False, 16, 32, 8, 1, True, True), ("bf16", False, 64, 8, 8, 3, True, True),
     ("f16", True, 32, 7, 1, 3, False, False), ("bf16", True, 16, 10, 2, 4, True, True),
@@ -263,7 +264,8 @@ def test_append_reports_bad_pages_and_positions(torch, P):
 
 
 # ------------------------------------------------------------------ read
-@pytest.mark.parametrize("q,kv,pad", [([1], [1], 0), ([33, 0, 100], [33, 3, 130], 5), ([50], [20], 0)])
+@pytest.mark.parametrize("q,kv,pad", [([1], [1], 0), ([33, 0, 100], [33, 3, 130], 5), ([50], [20], 0),
+                                      ([0, 0] + [b % 3 for b in range(1500)], [4] * 1502, 1)])
 @pytest.mark.parametrize("dtype,quant,page,hkv", [("f16", False, 16, 8), ("bf16", False, 256, 3), ("f16", True, 32, 1),
                                                   ("bf16", True, 64, 8)])
 def test_read(torch, P, q, kv, pad, dtype, quant, page, hkv):
@@ -325,6 +327,8 @@ LENGTHS = [
     ([33], [33]), ([64, 17, 0, 1], [200, 17, 3, 900]), ([130], [130]), ([257, 3], [1300, 5]), ([40, 40], [10, 0]),
     ([5] * 20, [1700 + 37 * b for b in range(20)]), ([1] * 20, [1701 + 37 * b for b in range(20)]),
     ([40] * 19, [900 + 41 * b for b in range(19)]),
+    ([(0, 1, 3, 2)[b % 4] for b in range(330)], [(7 * b) % 50 for b in range(330)]),
+    ([(1, 0, 45, 1, 2)[b % 5] for b in range(330)], [30 + b % 60 for b in range(330)]),
 ]
 
 
@@ -537,6 +541,19 @@ def test_verify(torch, P, dtype, V, with_probs):
     u = torch.rand((R + 12,), generator=g, device="cuda")
     check_verify(torch, P, logits.to(dtype_of(torch, dtype)), ids, start, [0.7, 1.0, 1.0, 0.3, 0.0, 2.0], u[:R], u[R:R + 6],
                  draft if with_probs else None)
+
+
+def test_verify_many_sequences(torch, P):
+    rows = [(1, 2, 0, 3)[b % 4] for b in range(150)]
+    g = gen(torch, 12)
+    start = [0]
+    for n in rows:
+        start.append(start[-1] + n)
+    R, B, V = start[-1], len(rows), 517
+    logits = torch.randn((R, V), generator=g, device="cuda") * 2
+    ids = logits.argmax(-1).roll(1).int()
+    u = torch.rand((R + B,), generator=g, device="cuda")
+    check_verify(torch, P, logits.half(), ids, start, [(0.0, 0.9, 1.3)[b % 3] for b in range(B)], u[:R], u[R:])
 
 
 def test_verify_greedy_ties_take_the_first_index(torch, P):
