@@ -140,7 +140,7 @@ dial_status dial_paged_attention(const void* q, const dial_paged_kv* kv, const d
 }
 
 size_t dial_verify_drafts_workspace_bytes(int64_t rows, int64_t vocab) {
-  if (rows <= 0 || vocab <= 0 || rows >= (1ll << 31) || vocab >= (1ll << 31)) return 0;
+  if (rows <= 0 || vocab <= 0 || rows >= (1ll << 31) || vocab > (1 << 30)) return 0;
   return verify_workspace_bytes(rows, vocab);
 }
 
@@ -156,8 +156,8 @@ dial_status dial_verify_drafts(const void* logits, dial_dtype dt, const int32_t*
   if (dt != DIAL_F32 && dt != DIAL_F16 && dt != DIAL_BF16) return fail(DIAL_ERR_UNSUPPORTED_DTYPE, "bad dtype");
   if (rows <= 0 || vocab <= 0 || n_seqs <= 0 || max_q <= 0)
     return fail(DIAL_ERR_INVALID_ARG, "sizes must be positive");
-  if (rows >= (1ll << 31) || vocab >= (1ll << 31) || n_seqs > (1 << 24) || max_q >= (1ll << 31))
-    return fail(DIAL_ERR_SHAPE, "rows, vocab and max_q must stay below 2^31");
+  if (rows >= (1ll << 31) || vocab > (1 << 30) || n_seqs > (1 << 24) || max_q >= (1ll << 31))
+    return fail(DIAL_ERR_SHAPE, "rows and max_q must stay below 2^31, vocab at most 2^30");
   const size_t need = verify_workspace_bytes(rows, vocab);
   if (workspace_bytes < need)
     return fail(DIAL_ERR_INVALID_ARG, "verification workspace must hold %zu bytes", need);

@@ -6,8 +6,8 @@
 //
 // Two launches, bound by reading the logits once (and, of one row a sequence, the
 // logits again from L2 and the draft's distribution):
-//   1. every row in segments of 1024, a warp each: maximum, first index of it, sum of e in f32,
-//      which decide the acceptances and give the log-probabilities;
+//   1. every row in segments of 1024, a warp each: maximum, its first index, sum of e in
+//      f32, which decide the acceptances and give the log-probabilities;
 //   2. a cluster of two to eight CTAs per sequence joins the segments, finds the first
 //      rejected draft and draws from that row.  The index at which a cumulative sum
 //      over 10^5 weights passes a random number moves with its last digits, so the
@@ -15,6 +15,9 @@
 //      short polynomial: P. T. P. Tang, ACM TOMS 15, 1989), eight f64 operations a
 //      value: every warp a run of the row, then the one run that the number falls in
 //      once more, element by element.
+// 32 sequences of up to 6 rows of 151936 in bf16 with the drafts' probabilities (47 MB)
+// take 32.7 us, 9.5 of them the segments, about 12 the f64 sweep; one sequence of 4 rows
+// takes 13.0 us, the chain of its steps.
 #include <algorithm>
 
 #include "common.cuh"
@@ -40,6 +43,16 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// (x - m) it of two values, two instructions
+__device__ __forceinline__ float2 octaves2(float x, float y, float minus_m, float it) {
+  float2 d;
+  asm("{\n .reg .b64 v, m, k;\n mov.b64 v, {%2, %3};\n mov.b64 m, {%4, %4};\n mov.b64 k, {%5, %5};\n"
+      " add.rn.f32x2 v, v, m;\n mul.rn.f32x2 v, v, k;\n mov.b64 {%0, %1}, v;\n}\n"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(x), "f"(y), "f"(minus_m), "f"(it));
+  return d;
 }
 
 // Aligned 16-byte vectors over an array of `total` elements; a row's elements [lo, hi)
@@ -124,11 +137,14 @@ __global__ void __launch_bounds__(kStatWarps * 32) verify_stats_kernel(VerifyArg
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
   float s = 0.f;
-  const float mt = -m * it;
+  // (the difference first: x it - m it would be off by 2^-24 |m| / T octaves)
 #pragma unroll
   for (int k = 0; k < PER; ++k)
 #pragma unroll
-    for (int i = 0; i < N; ++i) s += ex2(fmaf(f[k][i], it, mt));
+    for (int i = 0; i < N; i += 2) {
+      const float2 y = octaves2(f[k][i], f[k][i + 1], -m, it);
+      s += ex2(y.x), s += ex2(y.y);
+    }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   if (!(s < INFINITY)) {  // NaN logits, an infinite maximum, or none
@@ -178,16 +194,21 @@ __device__ const double kPow2[64] = {
     0x1.ea4afa2a490dap+0, 0x1.efa1bee615a27p+0, 0x1.f50765b6e4540p+0, 0x1.fa7c1819e90d8p+0};
 
 // exp((x - m) / T) up to a factor that all of a row share, to 2^-34, in eight f64
-// operations.  Values 1000 octaves below the maximum, minus infinity and NaN give 2^-1000,
-// which no sum feels and kNone tells from a weight.  Every lane has a copy of the table in
-// its own banks: entry j of lane l at table[32 j + l].
-constexpr double kNone = 1e-290;
+// operations.  Values 672 T or more below the maximum, minus infinity and NaN give what
+// `least` gives, 2^-970 up to `least`'s own rounding, 32 T or 46 octaves where T is 2^-29 |m|
+// (kSharp: below it they are not asked for).  No sum feels that, and kNone, above 2^30 times
+// 2^-923, tells it from a weight.  Every lane has a copy of the table in its own banks: entry
+// j of lane l at table[32 j + l].
+constexpr double kNone = 1e-268;
+// A row whose T is below kSharp |m|: the next f32 below m is 32 T or more away and weighs
+// less than 2^-46, so that the maximum takes everything.
+constexpr float kSharp = 0x1p-29f;
 struct Exp {
   const double* table;  // 2^(j / 64), this lane's
   double k, c;          // 64 log2(e) / T, minus m times that
   float least;
   __device__ __forceinline__ Exp(const double* t, float m, float temp, double k64)
-      : table(t + (threadIdx.x & 31)), k(k64), c(-(double)m * k64), least(fmaxf(m - 693.f * temp, -3e38f)) {}
+      : table(t + (threadIdx.x & 31)), k(k64), c(-(double)m * k64), least(fmaxf(m - 672.f * temp, -3e38f)) {}
   __device__ __forceinline__ double operator()(float x) const {
     const double y = fma((double)fmaxf(x, least), k, c);
     const double t = y + 6755399441055744.0;            // 1.5 * 2^52: the integer in the low word
@@ -387,8 +408,8 @@ __global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(kDrawThreads, PER_S
   }
 
   // ---- the draw from row `stop`: run w of CL * kWarps, in whole vectors
-  const bool inf = m == INFINITY;  // takes everything: weights 1 at the maximum
-  const Exp ex(table, inf ? 0.f : m, temp, k64);
+  const bool sharp = temp < kSharp * fabsf(m);  // (an infinite one too) weights 1 at the maximum
+  const Exp ex(table, sharp ? 0.f : m, temp, k64);
   // (vectors counted from the row's first, which like its last may hold other rows' values)
   const int64_t lo = stop * V, hi = lo + V, v0 = lo / N;
   const int nv = (int)((hi + N - 1) / N - v0), per = (nv + CL * kWarps - 1) / (CL * kWarps);
@@ -412,7 +433,7 @@ __global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(kDrawThreads, PER_S
 #pragma unroll
       for (int i = 0; i < N; ++i) f[i] = Act<T>::to_f32(h[i]);
     }
-    if (inf) {
+    if (sharp) {
 #pragma unroll
       for (int i = 0; i < N; ++i) f[i] = f[i] == m ? 0.f : -INFINITY;
     }
@@ -436,7 +457,7 @@ __global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(kDrawThreads, PER_S
   };
   auto weight1 = [&](int64_t e) {  // of one element of the row
     float f = Act<T>::to_f32(x[e]);
-    if (inf) f = f == m ? 0.f : -INFINITY;
+    if (sharp) f = f == m ? 0.f : -INFINITY;
     if (mode == 1 && e - lo == draft) f = -INFINITY;
     const double w = ex(f);
     if (mode < 2) return w;

@@ -508,7 +508,9 @@ DIAL_API dial_status dial_paged_attention(const void* q, const dial_paged_kv* kv
  * a sequence without rows); logprobs[r] (optional) = log p of it (temperature 1 for
  * 0), 0 where out_ids is -1.  A NaN logit counts as minus infinity; of a row
  * without any probability token 0 is drawn, with logprob -inf; an infinite logit
- * takes all of it.  A draft outside the vocabulary is rejected.  max_q: no sequence
+ * takes all of it, and so does the largest where the temperature is below 2^-29 of it
+ * (f32 neighbours are e^32 apart there); weights below 2^-890 of the largest count as
+ * none.  A draft outside the vocabulary is rejected.  vocab <= 2^30.  max_q: no sequence
  * has more rows (a longer one, or a q_start that falls or passes `rows`, sets the
  * device error flag).  logits and draft_probs are 16-byte aligned; rows of any
  * length.  `workspace`: dial_verify_drafts_workspace_bytes(rows, vocab)

@@ -92,6 +92,7 @@ def test_bad_verification_arguments():
     assert verify(dt=5) == 2
     assert verify(rows=0) == 1 and verify(vocab=0) == 1 and verify(n=0) == 1 and verify(max_q=0) == 1
     assert verify(rows=1 << 31) == 4 and verify(vocab=1 << 31) == 4
+    assert verify(vocab=(1 << 30) + 1) == 4 and D.lib().dial_verify_drafts_workspace_bytes(8, (1 << 30) + 1) == 0
     need = D.lib().dial_verify_drafts_workspace_bytes(8, 100)
     assert need > 0 and verify(nbytes=need - 1) == 1
     assert b"workspace" in D.lib().dial_last_error()

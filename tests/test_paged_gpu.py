@@ -556,6 +556,31 @@ def test_verify_many_sequences(torch, P):
     check_verify(torch, P, logits.half(), ids, start, [(0.0, 0.9, 1.3)[b % 3] for b in range(B)], u[:R], u[R:])
 
 
+@pytest.mark.parametrize("T", [0.2, 0.01, 1e-3, 2e-5, 1e-6, 2e-7, 1e-8, 2e-9, 3e-10, 1e-20, 1e-38, 1.4e-45])
+@pytest.mark.parametrize("dtype,offset", [("f32", 0), ("f32", -700), ("f16", 50), ("bf16", 0)])
+@pytest.mark.parametrize("with_probs", [False, True])
+def test_verify_cold(torch, P, T, dtype, offset, with_probs):
+    """Temperatures down to the least positive one: masked logits stay undrawn, near ones keep
+    their odds, ties share."""
+    rows = [1, 1, 3, 2, 1, 4, 1, 2, 5, 1]
+    g = gen(torch, 77)
+    start = [0]
+    for n in rows:
+        start.append(start[-1] + n)
+    R, V = start[-1], 3001
+    logits = (torch.randn((R, V), generator=g, device="cuda") + offset).to(dtype_of(torch, dtype))
+    near = logits.amax(-1, keepdim=True).double() - T * 3 * torch.rand((R, 40), generator=g, device="cuda").double()
+    at = torch.randperm(V, generator=g, device="cuda")
+    logits[:, at[:40]] = near.to(logits.dtype)  # of the largest one's order, some tied with it
+    logits[:, at[40:1500]] = -math.inf
+    draft = torch.rand((R, V), generator=g, device="cuda")
+    draft[:, at[40:]] *= 1e-3
+    draft /= draft.sum(-1, keepdim=True)
+    ids = at[torch.randint(0, 40, (R,), generator=g, device="cuda")].int()
+    u = torch.rand((R + len(rows),), generator=g, device="cuda")
+    check_verify(torch, P, logits, ids, start, [T] * len(rows), u[:R], u[R:], draft if with_probs else None)
+
+
 def test_verify_greedy_ties_take_the_first_index(torch, P):
     logits = torch.zeros((4, 999), device="cuda").half()
     logits[0, [5, 700]] = 3
