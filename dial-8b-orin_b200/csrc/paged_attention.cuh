@@ -152,7 +152,7 @@ __device__ __noinline__ void attend_row(const PagedView& p, int b, int g, int le
     for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
     s *= c;
     const float mn = fmaxf(m, s);
-    const float f = mn == m ? 1.f : exp2f(m - mn), e = exp2f(s - mn);
+    const float f = mn == m ? 1.f : exp2f(m - mn), e = s == -INFINITY ? 0.f : exp2f(s - mn);
     m = mn;
     l = l * f + e;
 #pragma unroll

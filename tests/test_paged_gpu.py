@@ -353,6 +353,25 @@ def test_attention_scale_and_peaked_rows(torch, P, quant, scale, q, kv):
     check_attention(torch, s, x, s.cache.attention(x, s.batch, scale=scale), scale=scale)
 
 
+@pytest.mark.parametrize("q,kv", [(2, 3), (5, 300), (60, 90), (40, 2000)])
+def test_a_key_of_minus_infinity_weighs_nothing_beside_unseen_nans(torch, P, q, kv):
+    """Scores of minus infinity in the rows that are computed again for an unseen NaN value."""
+    s = Setup(torch, P, [q], [kv], "f16", False, 16, 2, seed=4)
+    x = torch.randn((q, 8, D), generator=gen(torch, 9), device="cuda").half()
+    x[..., 0] = 1
+    s.pages[0][s.host_table[0][0], :, 0, 0] = -math.inf
+    want = torch.empty_like(x)
+    s.cache.attention(x, s.batch, out=want)
+    check_attention(torch, s, x, want)
+    s.pages[1][s.host_table[0][(kv - 1) // 16], :, (kv - 1) % 16] = math.nan
+    got = s.cache.attention(x, s.batch)
+    assert torch.isnan(got[-1]).all()
+    s.pages[1][s.host_table[0][(kv - 1) // 16], :, (kv - 1) % 16] = 0
+    want, size = attention64(torch, s, x, D ** -0.5)
+    off = (got[:-1].double() - want[:-1]).abs()
+    assert torch.all(off <= 2.0 ** -11 * want[:-1].abs() + (2.0 ** -11 + 2.0 ** -12) * size[:-1] + 1e-7)
+
+
 @pytest.mark.parametrize("q,kv", [([6], [300]), ([70, 40], [300, 141])])
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
 @pytest.mark.parametrize("quant", [False, True])
