@@ -49,6 +49,12 @@ dial_status find_flag(int** err) {
   return *err ? DIAL_OK : fail(DIAL_ERR_CUDA, "device error flag unavailable");
 }
 
+// Whether [a, a + n) and [b, b + m) (bytes) share any.
+bool overlap(const void* a, int64_t n, const void* b, int64_t m) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return x < y ? y - x < (uint64_t)n : x - y < (uint64_t)m;
+}
+
 dial_status check_heads(int hq, int hkv) {
   if (hq <= 0 || hq % hkv || hq / hkv > 8)
     return fail(DIAL_ERR_SHAPE, "heads must satisfy Hq %% Hkv == 0 and Hq/Hkv <= 8 (%d, %d)", hq, hkv);
@@ -107,6 +113,9 @@ dial_status dial_paged_kv_append(const void* qkv, const void* q_norm_w, const vo
   if (!aligned16(qkv) || !aligned16(q_out) || !aligned16(q_norm_w) || !aligned16(k_norm_w) ||
       !aligned16(cos_t) || !aligned16(sin_t))
     return fail(DIAL_ERR_MISALIGNED, "qkv, q_out, norm weights and tables must be 16-byte aligned");
+  const int64_t row = 256 * tokens;  // of one head, bytes
+  if (overlap(qkv, row * (n_heads + 2 * p.hkv), q_out, row * n_heads))
+    return fail(DIAL_ERR_INVALID_ARG, "q_out must not overlap qkv");
   if ((s = find_flag(&p.err)) != DIAL_OK) return s;
   return launch_paged_append(qkv, r, p, kv->format, q_out, dt, n_heads, as_stream(stream));
 }
@@ -120,6 +129,8 @@ dial_status dial_paged_kv_read(const dial_paged_kv* kv, const dial_paged_batch* 
   if (s != DIAL_OK) return s;
   if (!aligned16(k_out) || !aligned16(v_out))
     return fail(DIAL_ERR_MISALIGNED, "k_out and v_out must be 16-byte aligned");
+  if (overlap(k_out, 256 * tokens * p.hkv, v_out, 256 * tokens * p.hkv))
+    return fail(DIAL_ERR_INVALID_ARG, "k_out and v_out must not overlap");
   if ((s = find_flag(&p.err)) != DIAL_OK) return s;
   return launch_paged_read(p, kv->format, k_out, v_out, dt, as_stream(stream));
 }
@@ -135,6 +146,8 @@ dial_status dial_paged_attention(const void* q, const dial_paged_kv* kv, const d
   if ((s = check_heads(n_heads, p.hkv)) != DIAL_OK) return s;
   if (!(scale > 0.f) || scale > 1e30f) return fail(DIAL_ERR_INVALID_ARG, "scale must be positive and finite");
   if (!aligned16(q) || !aligned16(out)) return fail(DIAL_ERR_MISALIGNED, "q and out must be 16-byte aligned");
+  if (overlap(q, 256 * tokens * n_heads, out, 256 * tokens * n_heads))
+    return fail(DIAL_ERR_INVALID_ARG, "out must not overlap q");
   if ((s = find_flag(&p.err)) != DIAL_OK) return s;
   return launch_paged_attention(q, p, kv->format, out, dt, n_heads, batch->max_kv, scale, as_stream(stream));
 }

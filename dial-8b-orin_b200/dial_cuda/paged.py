@@ -100,7 +100,8 @@ class PagedBatch:
     tokens' counted), q_start int32 [n_seqs + 1] (token rows of each chunk).  max_q and
     max_kv are host-side bounds of a chunk and of kv_len (the largest possible by
     default); a chunk must not pass max_q, max_kv only sizes the work split.
-    The tensors may be rewritten between calls; the object keeps them alive."""
+    The tensors may be rewritten in place between calls (the object keeps them alive);
+    other tensors or bounds take a new object."""
 
     def __init__(self, block_table, kv_len, q_start, max_q: Optional[int] = None, max_kv: Optional[int] = None):
         torch = _torch()

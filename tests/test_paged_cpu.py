@@ -87,6 +87,17 @@ def test_bad_append_arguments():
     assert D.lib().dial_paged_kv_append(FAKE, None, None, FAKE, FAKE, 10, FAKE, None, kv(), batch(), FAKE, D.F16, 8, 32, 1e-6, None) == 1
 
 
+def test_overlapping_results():
+    L, at = D.lib(), lambda n: ctypes.c_void_p(0x10000 + n)
+    size = 8 * 32 * 256
+    for out in (at(0), at(size - 16), at(-size + 16)):
+        assert attention(q=at(0), out=out) == 1 and b"overlap" in L.dial_last_error()
+    for out in (at(0), at(8 * 8 * 256 - 16), at(-8 * 8 * 256 + 16)):
+        assert L.dial_paged_kv_read(kv(), batch(), at(0), out, D.F16, 8, None) == 1 and b"overlap" in L.dial_last_error()
+    for x in (FAKE, ctypes.c_void_p(0x1000 + size - 16), ctypes.c_void_p(0x1010)):
+        assert append(qkv=x) == 1 and b"overlap" in L.dial_last_error()
+
+
 def test_bad_verification_arguments():
     assert verify(logits=None) == 1 and verify(ids=None) == 1 and verify(ws=None) == 1
     assert verify(dt=5) == 2
