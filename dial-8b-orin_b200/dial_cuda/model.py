@@ -21,7 +21,7 @@ from typing import Optional
 
 from . import (BF16, F16, F32, GgufLinear, W8A16Linear, _torch, check, dtype_code, lib,
                stream_ptr)
-from .paged import PagedKVCache
+from .paged import PagedKVCache, _tensor
 
 WFMT_W8A16, WFMT_W8A16_F16S, WFMT_Q4_0, WFMT_Q8_0 = 0, 1, 2, 8
 
@@ -266,6 +266,9 @@ class Stage:
         behind the batch's last token come out unspecified."""
         torch = _torch()
         c, T = self.cfg, hidden.shape[0]
+        _tensor(hidden, "hidden", self.dt, (T, c.hidden), max(hidden.get_device(), 0))
+        if len(caches) != self.last - self.first:
+            raise ValueError(f"{self.last - self.first} layers take as many caches, got {len(caches)}")
         x, delta = torch.empty_like(hidden), None
         qkv = torch.empty((T, (c.n_heads + 2 * c.n_kv_heads) * c.head_dim), dtype=self.dt, device=self.device)
         q, attn = (torch.zeros((T, c.n_heads, c.head_dim), dtype=self.dt, device=self.device) for _ in range(2))
@@ -386,6 +389,7 @@ class Decoder:
         what `verify_drafts` takes, with the same ids and `batch.q_start`."""
         torch = _torch()
         st, T = self.stage, ids.numel()
+        _tensor(ids, "ids", torch.int32, (T,), max(ids.get_device(), 0))
         hidden = torch.empty((T, self.cfg.hidden), device=st.device, dtype=st.dt)
         st.embed_tokens(ids, hidden)
         st.layers_forward_paged(hidden, positions, batch, caches, tables, sections, interleaved)

@@ -831,6 +831,11 @@ def test_decoder_over_pages(torch, P, act, quant):
     caches = dec.stage.paged_caches(10, 16, quant)
     tables = P.rope_tables(128, cfg.rope_theta)
     table = torch.tensor([[4, 9, 1], [0, 7, 3]], **i32)
+    one = P.PagedBatch(table[:1], torch.tensor([1], **i32), torch.tensor([0, 1], **i32))
+    with pytest.raises(ValueError, match="caches"):
+        dec.forward_paged(seqs[0][:1], torch.zeros(1, **i32), one, caches[:1], tables)
+    with pytest.raises(TypeError, match="ids"):
+        dec.forward_paged(seqs[0][:1].long(), torch.zeros(1, **i32), one, caches, tables)
 
     def chunk(spans):
         ids = torch.cat([seqs[b][lo:hi] for b, (lo, hi) in enumerate(spans)])
