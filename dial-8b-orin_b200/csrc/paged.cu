@@ -65,9 +65,10 @@ __device__ __forceinline__ uint32_t code(float x, float inv) {
 // cosines, then walks heads, the next ones' values on their way while it works on four.
 // Few tokens: a head per eight lanes once; many: as few warps a token as fill the SMs, as
 // the look-ups cost about what four heads do.  2048 tokens of 32 + 2 * 8 heads in bf16 take
-// 15.5 us (50 MB, 3.2 TB/s), half of it what the bytes need; bound by instruction issue, the
-// sums in f64 and the packing above all.  A warp per head took 28.6 us, a warp per token
-// with two heads in it 15.8.
+// 15.5 us (50 MB, 3.2 TB/s), twice what the bytes need; bound by the chain of a head's steps
+// (sum, exchange, root, turn, pack) over two CTAs an SM: issue 40 %, and two or three heads
+// on their way instead of one change nothing.  A warp per head took 28.6 us, a warp per
+// token with two heads in it 15.8.
 // The mean square is summed in f64 (its squares are exact there) and 1/sqrt refined by one
 // Newton step in f64, so that the f32 factor -- and with it every int8 code -- does not
 // depend on the order of a sum; each later product is rounded to f32 on its own for the

@@ -25,6 +25,9 @@
 //   log2 v_s in the exponent, 1 / v_s in the row sum.
 // The warps' (m, l, O) meet in shared memory, the CTAs' in the cluster's: no
 // workspace, no counters, and the same result whatever the timing.
+// 32 sequences of 2049 int8 rows (8 kv heads, one token each) take 33 us (139 MB, 4.2 TB/s,
+// 20 us of it streaming); 16 with 5 tokens over up to 8200 bf16 rows 48 us (233 MB, 4.9
+// TB/s); one sequence of 2049 f16 rows 7.6 us, the chain length, page, tile, meeting.
 #include <cuda.h>
 
 #include <algorithm>
