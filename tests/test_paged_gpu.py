@@ -660,6 +660,58 @@ def test_verify_reports_bad_row_ranges(torch, P):
         assert device_error() == 1, start
 
 
+@pytest.mark.parametrize("T", [-1.0, -math.inf, math.nan])
+def test_verify_temperatures_that_are_not_positive_are_greedy(torch, P, T):
+    g = gen(torch, 31)
+    logits = torch.randn((7, 2100), generator=g, device="cuda").bfloat16()
+    ids = logits.argmax(-1).roll(1).int()
+    ids[6] += 1
+    u = torch.rand((10,), generator=g, device="cuda")
+    run = lambda t: run_verify(torch, P, logits, ids, [0, 3, 3, 7], [t] * 3, u[:7], u[7:])
+    for a, b in zip(run(T), run(0.0)):
+        assert torch.equal(a, b)
+
+
+def test_verify_numbers_outside_their_range_stay_inside_the_vocabulary(torch, P):
+    """u of 1, above, below 0 and NaN, draft weights that are NaN or infinite: some token that has
+    a probability is drawn."""
+    logits = torch.randn((12, 777), generator=gen(torch, 32), device="cuda")
+    logits[:, ::3] = -math.inf
+    ids = torch.full((12,), 4, dtype=torch.int32, device="cuda")
+    draft = torch.zeros((12, 777), device="cuda")
+    draft[:, 5], draft[:, 7], draft[:, 8] = math.nan, math.inf, -1.0
+    u = torch.tensor([1.0, 7.0, -2.0, math.nan, 1 - 2.0 ** -24, math.inf], device="cuda")
+    for probs in (None, draft):
+        out, count, logp = run_verify(torch, P, logits, ids, [0, 2, 4, 6, 8, 10, 12], [1.0] * 6, u.repeat(2), u, probs)
+        for b in range(6):
+            told = out[2 * b:2 * b + int(count[b])]
+            assert 1 <= int(count[b]) <= 2 and torch.all((told >= 0) & (told < 777) & (told % 3 != 0))
+
+
+def test_calls_on_several_streams_at_once(torch, P):
+    """Calls on streams of their own, over shared and other caches, give the bits of calls in turn."""
+    s = Setup(torch, P, [3, 60, 1], [300, 700, 2000], "bf16", True, 32, 4, seed=8)
+    d = Setup(torch, P, [1] * 6, [100 * b + 9 for b in range(6)], "bf16", True, 32, 4, seed=9)
+    g = gen(torch, 33)
+    x, y = (torch.randn((z.T, 16, D), generator=g, device="cuda").bfloat16() for z in (s, d))
+    logits = torch.randn((s.T, 9001), generator=g, device="cuda")
+    ids, u = logits.argmax(-1).roll(1).int(), torch.rand((s.T + 3,), generator=g, device="cuda")
+    temp = torch.tensor([0.0, 0.8, 1.5], device="cuda")
+    calls = [lambda: s.cache.attention(x, s.batch), lambda: d.cache.attention(y, d.batch), lambda: s.cache.read(s.batch, s.T)[0],
+             lambda: P.verify_drafts(logits, ids, s.q_start, temp, u[:s.T], u[s.T:])[0][:s.start[-1]]]
+    want = [f() for f in calls]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in calls]
+    got = []
+    for _ in range(10):
+        for f, st in zip(calls, streams):
+            with torch.cuda.stream(st):
+                got.append(f())
+    torch.cuda.synchronize()
+    for i, z in enumerate(got):
+        assert torch.equal(z, want[i % len(calls)])
+
+
 def test_verify_in_graphs(torch, P):
     g = gen(torch, 1)
     R, V = 8, 151936
