@@ -26,18 +26,11 @@ SECTIONS = {1: (64,), 2: (40, 24), 3: (24, 20, 20), 4: (16, 16, 16, 16)}
 DTYPES = {"f16": torch.float16, "bf16": torch.bfloat16, "f32": torch.float32}
 
 
-_paged = None
-
-
 def _framework():
-    global _paged
-    if _paged is not None:
-        return _paged
     at = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "dial-8b-orin_b200")
     if at not in sys.path:
         sys.path.insert(0, at)
     from dial_cuda import paged
-    _paged = paged
     return paged
 
 
