@@ -454,6 +454,12 @@ __global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(kDrawThreads, PER_S
 #pragma unroll
       for (int i = 0; i < N; ++i) q[i] = (v0 + v) * N + i < total ? qv[v * N + i] : 0.f;
     }
+    if (v == 0 || v == nv - 1) {  // other rows' values, whatever they are, are none of this row's
+      const int64_t e = (v0 + v) * N;
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (e + i < lo || e + i >= hi) q[i] = 0.f;
+    }
   };
   auto weight1 = [&](int64_t e) {  // of one element of the row
     float f = Act<T>::to_f32(x[e]);
@@ -504,7 +510,7 @@ __global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(kDrawThreads, PER_S
           if (v < a1) {
             float f[N];
             values(held[k][threadIdx.x], v, f);
-            if (mode >= 2) {  // (outside the row e is nothing, and not above q z0 unless q is 0)
+            if (mode >= 2) {  // (outside the row e is nothing and q is 0)
               float q[N];
               draft_probs(v, q);
               const double z = mode == 3 ? z0 : z64;

@@ -499,7 +499,9 @@ DIAL_API dial_status dial_paged_attention(const void* q, const dial_paged_kv* kv
  * of logits [rows, vocab] (f32, f16 or bf16) and of ids (the chunk the target model
  * was run on: its last accepted token, then the drafts), so row r judges draft
  * ids[r + 1] unless it is the sequence's last.  p = softmax(logits / temperature[b]);
- * q = row r of draft_probs [rows, vocab] (f32), or NULL: the drafts were certain.
+ * q = row r of draft_probs [rows, vocab] (f32), or NULL: the drafts were certain (the
+ * rows that judge no draft, each sequence's last and those behind the last sequence,
+ * may hold anything).
  * In order, a draft x is accepted if accept_u[r] * q(x) < p(x) (u in [0, 1)); at the
  * first that is not, a token is drawn from max(p - q, 0) (p if nothing is left of
  * it), and behind the last draft one from p: the first index whose cumulative

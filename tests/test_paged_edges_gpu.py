@@ -1,0 +1,50 @@
+"""Edges of the paged-cache operators on the GPU: what stands beside a row in memory,
+weights at the ends of their range, and calls that share memory.  Tolerances are those of
+test_paged_gpu.py, or equality of bits."""
+import math
+
+import pytest
+
+from test_paged_gpu import (D, Setup, attention64, check_attention, check_verify, device_error, dtype_of, gen,  # noqa: F401
+                            no_device_error, run_verify)
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def torch(cuda):
+    import torch as _t
+    return _t
+
+
+@pytest.fixture(scope="module")
+def P(cuda):
+    from dial_cuda import paged
+    return paged
+
+
+# ------------------------------------------------------------------ verification
+@pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("V", [7, 777, 4099])
+@pytest.mark.parametrize("bad", [math.nan, -0.05, -1e30, math.inf, -math.inf])
+def test_draft_probs_of_rows_that_judge_no_draft_are_not_read(torch, P, dtype, V, bad):
+    """A row of odd length shares its first and last vectors with its neighbours: the draft's
+    weights in a sequence's last row and behind the last sequence may hold anything."""
+    rows = [1, 2, 4, 0, 2, 3, 1, 2, 2, 5]
+    g = gen(torch, V)
+    start = [0]
+    for n in rows:
+        start.append(start[-1] + n)
+    R = start[-1] + 2
+    logits = (torch.randn((R, V), generator=g, device="cuda") * 2).to(dtype_of(torch, dtype))
+    draft = (logits.float() + torch.randn((R, V), generator=g, device="cuda")).softmax(-1)
+    idle = [e - 1 for e, n in zip(start[1:], rows) if n] + [R - 2, R - 1]
+    draft[idle] = 0
+    ids = torch.randint(0, V, (R,), generator=g, device="cuda", dtype=torch.int32)
+    u = torch.rand((len(rows),), generator=g, device="cuda")
+    accept = torch.full((R,), 0.999, device="cuda")
+    want = check_verify(torch, P, logits, ids, start, [1.0] * len(rows), accept, u, draft)
+    draft[idle] = bad
+    got = run_verify(torch, P, logits, ids, start, [1.0] * len(rows), accept, u, draft)
+    n = start[-1]
+    assert torch.equal(got[0][:n], want[0][:n]) and torch.equal(got[1], want[1]) and torch.equal(got[2][:n], want[2][:n])
