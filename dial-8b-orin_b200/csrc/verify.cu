@@ -197,9 +197,11 @@ __device__ const double kPow2[64] = {
 // operations.  Values 672 T or more below the maximum, minus infinity and NaN give what
 // `least` gives, 2^-970 up to `least`'s own rounding, 32 T or 46 octaves where T is 2^-29 |m|
 // (kSharp: below it they are not asked for).  No sum feels that, and kNone, above 2^30 times
-// 2^-923, tells it from a weight.  Every lane has a copy of the table in its own banks: entry
-// j of lane l at table[32 j + l].
-constexpr double kNone = 1e-268;
+// 2^-923, tells it from a weight: a run's sum above kNone is one.  The run has fewer than 2^24
+// vectors, so one of them is above kNoneVec then, and of its at most eight elements one is above
+// kNoneOne, still 2^6 times what `least` gives.  Every lane has a copy of the table in its own
+// banks: entry j of lane l at table[32 j + l].
+constexpr double kNone = 0x1p-890, kNoneVec = 0x1p-914, kNoneOne = 0x1p-917;
 // A row whose T is below kSharp |m|: the next f32 below m is 32 T or more away and weighs
 // less than 2^-46, so that the maximum takes everything.
 constexpr float kSharp = 0x1p-29f;
@@ -550,8 +552,8 @@ __global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(kDrawThreads, PER_S
           const double y = __shfl_up_sync(0xffffffffu, pre, o);
           if (lane >= o) pre += y;
         }
-        const unsigned some = __ballot_sync(0xffffffffu, s > kNone && cum + pre > at);
-        const unsigned any = __ballot_sync(0xffffffffu, s > kNone);
+        const unsigned some = __ballot_sync(0xffffffffu, s > kNoneVec && cum + pre > at);
+        const unsigned any = __ballot_sync(0xffffffffu, s > kNoneVec);
         if (any) {
           const int l = some ? __ffs(some) - 1 : 31 - __clz(any);
           vec = c0 + 32 * k + l;
@@ -569,9 +571,9 @@ __global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(kDrawThreads, PER_S
           const double y = __shfl_up_sync(0xffffffffu, pre, o);
           if (lane >= o) pre += y;
         }
-        const unsigned some = __ballot_sync(0xffffffffu, w > kNone && start + pre > at);
-        const unsigned any = __ballot_sync(0xffffffffu, w > kNone);
-        token = (int)((v0 + vec) * N + (some ? __ffs(some) - 1 : 31 - __clz(any)) - lo);
+        const unsigned some = __ballot_sync(0xffffffffu, w > kNoneOne && start + pre > at);
+        const unsigned any = __ballot_sync(0xffffffffu, w > kNoneOne);
+        if (any) token = (int)((v0 + vec) * N + (some ? __ffs(some) - 1 : 31 - __clz(any)) - lo);
       }
     }
     if (locate) break;
@@ -594,7 +596,11 @@ __global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(kDrawThreads, PER_S
     }
   }
   if (run >= 0) {
-    token = token < 0 ? top : token;
+    // (sums of max(p - q, 0) that rounding alone raised above zero leave no element: the maximum)
+    for (int64_t e = lane; token < 0 && e - lane < V; e += 32) {
+      const unsigned at_max = __ballot_sync(0xffffffffu, e < V && Act<T>::to_f32(x[lo + min(e, V - 1)]) == m);
+      if (at_max) token = (int)(e - lane) + __ffs(at_max) - 1;
+    }
     if (lane == 0) tell(token, Act<T>::to_f32(x[lo + token]));
   }
   __syncwarp();

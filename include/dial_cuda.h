@@ -515,7 +515,7 @@ DIAL_API dial_status dial_paged_attention(const void* q, const dial_paged_kv* kv
  * without any probability token 0 is drawn, with logprob -inf; an infinite logit
  * takes all of it, and so does the largest where the temperature is below 2^-29 of it
  * (f32 neighbours are e^32 apart there); weights below 2^-890 of the largest count as
- * none.  A draft outside the vocabulary is rejected.  vocab <= 2^30.  max_q: no sequence
+ * none (or, where several of them together pass it, as they are).  A draft outside the vocabulary is rejected.  vocab <= 2^30.  max_q: no sequence
  * has more rows (a longer one, or a q_start that falls or passes `rows`, sets the
  * device error flag).  logits and draft_probs are 16-byte aligned; rows of any
  * length.  `workspace`: dial_verify_drafts_workspace_bytes(rows, vocab)

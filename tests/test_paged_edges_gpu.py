@@ -48,3 +48,19 @@ def test_draft_probs_of_rows_that_judge_no_draft_are_not_read(torch, P, dtype, V
     got = run_verify(torch, P, logits, ids, start, [1.0] * len(rows), accept, u, draft)
     n = start[-1]
     assert torch.equal(got[0][:n], want[0][:n]) and torch.equal(got[1], want[1]) and torch.equal(got[2][:n], want[2][:n])
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("rows", [1, 2])
+@pytest.mark.parametrize("step", [1, 7, 13])
+@pytest.mark.parametrize("V", [1000, 151936])
+def test_weights_that_count_only_together_draw_one_of_their_own(torch, P, dtype, rows, step, V):
+    """Eight weights of e^-617.3, each below 2^-890 of the maximum's and above it as a sum, in one
+    vector or several: with u = 0 one of them or the maximum is drawn, none without probability."""
+    logits = torch.full((rows, V), -math.inf, device="cuda")
+    at = 16 + step * torch.arange(8, device="cuda")
+    logits[:, at] = -1
+    logits[:, 900] = 0
+    got = run_verify(torch, P, logits.to(dtype_of(torch, dtype)), [2] * rows, [0, rows], [1 / 617.3], [0.5] * rows, [0.0])
+    assert int(got[0][0]) in at.tolist() + [900]
+    assert got[1].tolist() == [1] and math.isfinite(float(got[2][0]))
