@@ -11,8 +11,8 @@
 //   2. a cluster of two to eight CTAs per sequence joins the segments, finds the first
 //      rejected draft and draws from that row.  The index at which a cumulative sum
 //      over 10^5 weights passes a random number moves with its last digits, so the
-//      draw sums in f64 over exponentials good to 2^-34 (a table of 2^(j/64) and a
-//      short polynomial: P. T. P. Tang, ACM TOMS 15, 1989), eight f64 operations a
+//      draw sums in f64 over exponentials good to 2^-44 (a table of 2^(j/64) and a
+//      short polynomial: P. T. P. Tang, ACM TOMS 15, 1989), nine f64 operations a
 //      value: every warp a run of the row, then the one run that the number falls in
 //      once more, element by element.
 // 32 sequences of up to 6 rows of 151936 in bf16 with the drafts' probabilities (47 MB)
@@ -193,8 +193,8 @@ __device__ const double kPow2[64] = {
     0x1.d5818dcfba487p+0, 0x1.da9e603db3285p+0, 0x1.dfc97337b9b5fp+0, 0x1.e502ee78b3ff6p+0,
     0x1.ea4afa2a490dap+0, 0x1.efa1bee615a27p+0, 0x1.f50765b6e4540p+0, 0x1.fa7c1819e90d8p+0};
 
-// exp((x - m) / T) up to a factor that all of a row share, to 2^-34, in eight f64
-// operations.  Values 672 T or more below the maximum, minus infinity and NaN give what
+// exp((x - m) / T) up to a factor that all of a row share, to 2^-44, in nine f64
+// operations (a cubic, good to 2^-34, leaves 2^-11 of a weight max(p - q, 0) of 2^-23 p).  Values 672 T or more below the maximum, minus infinity and NaN give what
 // `least` gives, 2^-970 up to `least`'s own rounding, 32 T or 46 octaves where T is 2^-29 |m|
 // (kSharp: below it they are not asked for).  No sum feels that, and kNone, above 2^30 times
 // 2^-923, tells it from a weight: a run's sum above kNone is one.  The run has fewer than 2^24
@@ -216,7 +216,8 @@ struct Exp {
     const double t = y + 6755399441055744.0;            // 1.5 * 2^52: the integer in the low word
     const int n = __double2loint(t);
     const double r = y - (t - 6755399441055744.0);
-    double p = 2.1173137155464774e-07;                  // (ln2 / 64)^j / j!
+    double p = 5.732851688640402e-10;                   // (ln2 / 64)^j / j!
+    p = fma(p, r, 2.1173137155464774e-07);
     p = fma(p, r, 5.864904955056169e-05);
     p = fma(p, r, 0.010830424696249145);
     const double e = table[(n & 63) * 32];
@@ -423,9 +424,13 @@ __global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(kDrawThreads, PER_S
   double z64 = 0.0;
   const double z0 = (double)Z;
   // 0: all of p; 1: p without the draft; 3: max(p - q, 0) Z = max(e - q Z, 0) in one pass, by
-  // the sums of e and q where e > q z0, z0 being Z as the segments gave it: a value on the
-  // wrong side of that has a weight below 2^-23 of its e, and nothing else depends on z0.
-  // Where little is left (below 2^-12 of p) 2 follows: the same with Z in f64 throughout.
+  // the sums of e and q where e > q z0, z0 being Z as the segments gave it in f32: off by
+  // 2^-23 of it or so, by 2^-17 at most (an exponent of 17 octaves has three roundings of
+  // 2^-24 of it, ex2 one of 2^-22, and a sum of 2^18 values goes through some 40 additions).
+  // Nothing else depends on z0, and a value on the wrong side of it has a weight of
+  // |e - q Z| <= q |z0 - Z|, all of them together |z0 - Z|.  Both are known after the pass:
+  // where what is left of p is not 2^16 times that (or below 2^-12 of p, which the difference
+  // of two sums would feel) 2 follows: the same with Z in f64 throughout.
   int mode = !rejected ? 0 : (a.probs ? 3 : 1);
   auto values = [&](uint4 u, int v, float (&f)[N]) {
     if (v == 0 || v == nv - 1) {
@@ -585,7 +590,7 @@ __global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(kDrawThreads, PER_S
     int r;
     all = meet<CL>(sum[buf], rank, mode == 3, mine, mina, minq, z64, u, r, before);
     buf ^= 1;
-    if (mode == 3 && !(all > z64 * 0x1p-12)) {
+    if (mode == 3 && !(all > fmax(z64 * 0x1p-12, fabs(z64 - z0) * 0x1p16))) {
       mode = 2;
     } else if (mode && mode != 3 && !(all > kNone)) {
       mode = 0;  // nothing left of it: from p

@@ -64,3 +64,26 @@ def test_weights_that_count_only_together_draw_one_of_their_own(torch, P, dtype,
     got = run_verify(torch, P, logits.to(dtype_of(torch, dtype)), [2] * rows, [0, rows], [1 / 617.3], [0.5] * rows, [0.0])
     assert int(got[0][0]) in at.tolist() + [900]
     assert got[1].tolist() == [1] and math.isfinite(float(got[2][0]))
+
+
+@pytest.mark.parametrize("T", [1.0, 0.6])
+@pytest.mark.parametrize("V", [1024, 9001])
+def test_a_draft_nearly_equal_to_the_target(torch, P, T, V):
+    """All of max(p - q, 0) but 2^-11.5 of it lies in weights of 2^-22.5 p, on which a sum of e in
+    f32 cannot decide: at u = 0 and little above the first of them are drawn, as defined."""
+    n = 64
+    g = gen(torch, V)
+    logits = torch.randn((2 * n, V), generator=g, device="cuda") * 2
+    logits[:, V - 1] = logits[:, :V - 2].amax(-1) + 1
+    p = (logits.double() / T).softmax(-1)
+    draft = p * (1 - 2.0 ** -22.5)
+    draft[:, V - 1] = p[:, V - 1] - 2.0 ** -11.5
+    draft[:, V - 2] = p[:, V - 2] + 2.0 ** -11.5
+    ids = torch.full((2 * n,), V - 2, dtype=torch.int32, device="cuda")
+    u = torch.cat([torch.zeros(n // 2, device="cuda"), torch.rand(n // 2, generator=g, device="cuda") * 2.0 ** -11])
+    temp = torch.full((n,), T, device="cuda")
+    p = (logits.double() / temp[0].double()).softmax(-1)
+    keep = (p[:, V - 2] < 0.9999 * draft[:, V - 2]).all()
+    assert keep  # the draft is refused
+    check_verify(torch, P, logits, ids, list(range(0, 2 * n + 1, 2)), temp, torch.full((2 * n,), 0.9999, device="cuda"), u,
+                 draft.float())
