@@ -14,7 +14,7 @@
 //   S^T [16 keys x 8 rows] = K Q^T,   O^T [16 dims x 8 rows] += V^T P^T;
 // S^T's 8 x 8 blocks become P^T's operand by movmatrix.  A row's maximum in use
 // moves only when a score passes it by 2^8 (a vote; the exchange over the lanes is
-// rare), and P stays below 2^8.
+// rare); P's range is in paged_attention.cuh.
 //   16-bit pages: 16 keys a tile, operands by ldmatrix (V transposed).
 //   int8 pages: 32 keys a tile, widened to f16 in registers.  The order of the 128
 //   dims in K Q^T is free as long as Q follows it: a lane takes 16 consecutive bytes
@@ -114,8 +114,8 @@ __global__ void __launch_bounds__((Cfg<Q8, NR>::WARPS * 32), (Cfg<Q8, NR>::PER_S
   constexpr int TK = L::TK, WARPS = L::WARPS, TILE = L::TILE, STAGE = L::STAGE, STAGES = L::STAGES;
   constexpr int KT = TK / 16;       // 16-key tiles of the scores
   constexpr int ROWS = 8 * NR;
-  constexpr float kGrow = 8.f;      // log2 growth of a row's maximum before it moves
   using MT = typename std::conditional<Q8, __half, T>::type;  // operands
+  constexpr float LIFT = kLift<MT>;
   extern __shared__ uint8_t smem_raw[];
   __shared__ float sm_m[WARPS][ROWS], sm_l[WARPS][ROWS], cta_m[ROWS], cta_l[ROWS];
   __shared__ __align__(8) uint64_t bars[WARPS * STAGES];
@@ -343,7 +343,7 @@ __global__ void __launch_bounds__((Cfg<Q8, NR>::WARPS * 32), (Cfg<Q8, NR>::PER_S
         float mx = fmaxf(sc[n][0][e], sc[n][0][2 + e]);
 #pragma unroll
         for (int x = 1; x < KT; ++x) mx = fmaxf(mx, fmaxf(sc[n][x][e], sc[n][x][2 + e]));
-        grow |= (Q8 ? mx : mx * c) > m[n][e] + kGrow;
+        grow |= (Q8 ? mx : mx * c) > m[n][e] + (kGrow + LIFT);
       }
     if (__any_sync(0xffffffffu, grow)) {  // rare: the rows' maxima move
 #pragma unroll
@@ -355,7 +355,7 @@ __global__ void __launch_bounds__((Cfg<Q8, NR>::WARPS * 32), (Cfg<Q8, NR>::PER_S
           for (int x = 0; x < KT; ++x) mx = fmaxf(mx, fmaxf(sc[n][x][e], sc[n][x][2 + e]));
 #pragma unroll
           for (int z = 4; z < 32; z <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, z));
-          const float mn = fmaxf(m[n][e], Q8 ? mx : mx * c);
+          const float mn = fmaxf(m[n][e], (Q8 ? mx : mx * c) - LIFT);
           const float f = m[n][e] == -INFINITY ? 0.f : ex2(m[n][e] - mn);
           m[n][e] = mn;
           l[n][e] *= f;

@@ -24,6 +24,16 @@ __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, int* err) {
     }
   }
 }
+// P is rounded once, to the 16 bits that the matrix instructions take; its sum is of the
+// unrounded values.  P = 2^(s - m) with m kLift below a maximum of the row, which moves when a
+// score passes it by kGrow more: f16 operands (and int8 pages, whose P carries the value's
+// scale) have P in [0, 2^15], so that a weight of 2^-21 of the row's largest still has its 11
+// bits and the last bit is 2^-31 of it.  From 1 instead of 2^7 on, 2048 keys 22 octaves below a
+// first one without a value were off by 2^-9.4 of their sum.  bf16's range needs no lift.
+constexpr float kGrow = 8.f;
+template <typename T>
+constexpr float kLift = std::is_same<T, __half>::value ? 7.f : 0.f;
+
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

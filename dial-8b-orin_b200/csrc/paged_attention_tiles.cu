@@ -10,13 +10,13 @@
 //               MN-major descriptor), f32 in TMEM
 // While a warpgroup turns S into P for one tile, the tensor cores work on the
 // other.  O is rescaled only when a row's maximum grew by more than 2^8 over the
-// one in use (P then stays below 2^8, and 16-bit rounding is relative), by the
+// one in use (P's range is in paged_attention.cuh), by the
 // thread that owns the row: S of a key tile is complete only after O += P V of
 // the tile before, so nothing else touches O then.
 //
 // int8 pages: a warpgroup widens the codes to 16 bits (exact).  The key's scale
 // multiplies its score column; the value's scale v goes into the exponent, P' =
-// 2^(c k_s S + log2 v - m'), so that P' stays in [0, 2^8] whatever the scales
+// 2^(c k_s S + log2 v - m'), so that P' stays in [0, 2^15] whatever the scales
 // are, and the row sum takes P' / v.
 //
 // TMEM (512 columns): S of the two tiles in [0, 256), O in [256, 512).
@@ -52,7 +52,6 @@ constexpr int QT = 128;             // rows per query tile
 constexpr int HALF = KT * 128;      // bytes of 128 rows x 64 dims of 16 bits
 constexpr int SLOT = 2 * HALF;      // one K or V tile
 constexpr int RAW = KT * 128;       // one int8 K or V tile
-constexpr float kGrow = 8.f;        // log2 growth of a row's maximum before O is rescaled
 
 template <bool Q8>
 struct Cfg {
@@ -200,6 +199,7 @@ __global__ void __launch_bounds__(Cfg<Q8>::THREADS, 1)
   using PT = typename std::conditional<Q8, __half, T>::type;  // operands of P V
   constexpr bool kBf = std::is_same<T, __nv_bfloat16>::value, kPBf = std::is_same<PT, __nv_bfloat16>::value;
   constexpr int NS = L::SLOTS;
+  constexpr float LIFT = kLift<PT>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t base = smem_u32(smem), bars = base + L::BAR_OFF;
@@ -488,9 +488,9 @@ __global__ void __launch_bounds__(Cfg<Q8>::THREADS, 1)
         float top = max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]);
         if (!Q8) top *= a.c;
         // the maximum in use moves only when the new one is far above it
-        const bool move = top > m + kGrow || (m == -INFINITY && top > m);
+        const bool move = top > m + (kGrow + LIFT) || (m == -INFINITY && top > m);
         if (__any_sync(0xffffffffu, move)) {
-          const float mn = move ? top : m;
+          const float mn = move ? top - LIFT : m;
           const float f = move && m != -INFINITY ? ex2(m - mn) : (move ? 0.f : 1.f);
           m = mn;
           l *= f;

@@ -488,7 +488,7 @@ DIAL_API dial_status dial_paged_kv_read(const dial_paged_kv* kv, const dial_page
  * attends the cache rows up to its own, out [T, Hq * 128] =
  * softmax(scale * q.K^T) V.  Rows that a token does not attend do not touch its
  * result, whatever they hold.  Needs no workspace; out must not overlap q.  Where a
- * value row that is not finite, or an int8 row's scale that is 0 or below 2^-100, sits
+ * value row that is not finite, or an int8 row's scale that is 0 or below 2^-90, sits
  * near a token's rows, that token is computed key by key, which is far slower. */
 DIAL_API dial_status dial_paged_attention(const void* q, const dial_paged_kv* kv,
                                           const dial_paged_batch* batch, void* out, dial_dtype dt,

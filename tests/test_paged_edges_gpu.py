@@ -87,3 +87,27 @@ def test_a_draft_nearly_equal_to_the_target(torch, P, T, V):
     assert keep  # the draft is refused
     check_verify(torch, P, logits, ids, list(range(0, 2 * n + 1, 2)), temp, torch.full((2 * n,), 0.9999, device="cuda"), u,
                  draft.float())
+
+
+# ------------------------------------------------------------------ attention
+@pytest.mark.parametrize("octaves", [18, 22, 24])
+@pytest.mark.parametrize("q,kv", [([1], [2049]), ([1, 2], [40001, 700]), ([5], [9000]), ([40], [2100]), ([300, 9], [2500, 5000])])
+@pytest.mark.parametrize("dtype,quant", [("f16", False), ("bf16", False), ("f16", True), ("bf16", True)])
+def test_a_first_key_that_takes_nearly_all_weight(torch, P, octaves, q, kv, dtype, quant):
+    """The first key `octaves` above all others, with a value row of zeros (int8: a small one, as zeros
+    have the scale 1): what the others leave is as exact as anywhere."""
+    s = Setup(torch, P, q, kv, dtype, quant, 64, 2, seed=octaves)
+    x = torch.randn((s.T, 8, D), generator=gen(torch, 5), device="cuda") * 0.3
+    x[..., 0] = 4
+    x = x.to(dtype_of(torch, dtype))
+    at = octaves / (4 * D ** -0.5 * math.log2(math.e))
+    s.pages[0][..., 0] = 0
+    for b in range(len(q)):
+        first = s.host_table[b][0]
+        s.pages[0][first, :, 0] = 0
+        s.pages[0][first, :, 0, 0] = 127 if quant else at
+        if quant:
+            s.scales[0][first, :, 0], s.scales[1][first, :, 0] = at / 127, 2.0 ** -12
+        else:
+            s.pages[1][first, :, 0] = 0
+    check_attention(torch, s, x, s.cache.attention(x, s.batch))
