@@ -236,7 +236,7 @@ __global__ void __launch_bounds__((Cfg<Q8, NR>::WARPS * 32), (Cfg<Q8, NR>::PER_S
         }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    const int e = min(max((int)(__float_as_uint(top) >> 23) - 127 - 10, -100), 100);
+    const int e = max((int)(__float_as_uint(top) >> 23) - 127 - 10, -100);  // up to 117
     const float down = __uint_as_float((uint32_t)(127 - e) << 23);
     c *= __uint_as_float((uint32_t)(127 + e) << 23);
 #pragma unroll

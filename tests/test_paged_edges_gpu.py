@@ -111,3 +111,15 @@ def test_a_first_key_that_takes_nearly_all_weight(torch, P, octaves, q, kv, dtyp
         else:
             s.pages[1][first, :, 0] = 0
     check_attention(torch, s, x, s.cache.attention(x, s.batch))
+
+
+@pytest.mark.parametrize("top", [2.0 ** 100, 2.0 ** 112, 2.0 ** 119, -2.0 ** 100, -2.0 ** 112, -2.0 ** 119, 2.0 ** -100, -2.0 ** -100])
+@pytest.mark.parametrize("q,kv", [([1], [50]), ([3], [2100]), ([30, 1], [99, 700])])
+def test_bf16_queries_at_the_ends_of_their_range_over_int8_pages(torch, P, top, q, kv):
+    """One large value a query, every score of one sign: the key with the largest takes all."""
+    s = Setup(torch, P, q, kv, "bf16", True, 32, 2)
+    x = torch.zeros((s.T, 8, D), device="cuda")
+    x[..., 3] = top
+    x = x.bfloat16()
+    s.pages[0].abs_().clamp_(min=1)
+    check_attention(torch, s, x, s.cache.attention(x, s.batch))
