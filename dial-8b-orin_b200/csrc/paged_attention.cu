@@ -491,6 +491,7 @@ __global__ void __launch_bounds__((Cfg<Q8, NR>::WARPS * 32), (Cfg<Q8, NR>::PER_S
     float M = -INFINITY, Ls = 0.f;
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
     if (S == 1) {
+      M = cta_m[r];
       Ls = cta_l[r];
       v = *reinterpret_cast<const float4*>(part + r * D + 4 * lane);
     } else {
@@ -517,7 +518,7 @@ __global__ void __launch_bounds__((Cfg<Q8, NR>::WARPS * 32), (Cfg<Q8, NR>::PER_S
     }
     const float w[4] = {Ls == 0.f ? 0.f : v.x / Ls, Ls == 0.f ? 0.f : v.y / Ls, Ls == 0.f ? 0.f : v.z / Ls,
                         Ls == 0.f ? 0.f : v.w / Ls};
-    bool fine = fabsf(Ls) < INFINITY;
+    bool fine = fabsf(Ls) < INFINITY && (Q8 || in_range<MT>(Ls, M));
 #pragma unroll
     for (int e = 0; e < 4; ++e) fine = fine && fabsf(w[e]) < INFINITY;
     const int64_t at = ((ch.q0 + i) * a.hq + g * a.rep + r % a.rep) * D;

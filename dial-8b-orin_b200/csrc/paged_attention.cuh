@@ -33,6 +33,14 @@ __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, int* err) {
 constexpr float kGrow = 8.f;
 template <typename T>
 constexpr float kLift = std::is_same<T, __half>::value ? 7.f : 0.f;
+// Whether a row's sum l, in units of its maximum m, came about in P's range.  Over 16-bit pages
+// m is a rounded product, c S, and P = 2^(c S - m) an exact difference: below 2^23 they agree to
+// half an octave, so that the row's largest P is 2^(LIFT - 1/2) or more.  Scores far above that
+// leave it anywhere, and a row whose largest P came out small is computed again.
+template <typename T>
+__device__ __forceinline__ bool in_range(float l, float m) {
+  return l >= (kLift<T> > 0.f ? 64.f : 0.5f) || m == -INFINITY;
+}
 
 __device__ __forceinline__ float ex2(float x) {
   float y;

@@ -580,7 +580,7 @@ __global__ void __launch_bounds__(Cfg<Q8>::THREADS, 1)
             }
           }
         }
-        fine = fine && fabsf(l) < INFINITY;
+        fine = fine && fabsf(l) < INFINITY && (Q8 || in_range<PT>(l, m));
       } else if (real) {  // a tile without any key
 #pragma unroll
         for (int e = 0; e < 16; ++e) reinterpret_cast<uint4*>(dst)[e] = make_uint4(0, 0, 0, 0);
@@ -632,6 +632,7 @@ __global__ void __launch_bounds__(Cfg<Q8>::THREADS, 1)
           const float mz = ld_cluster(mapa(at, z)), lz = ld_cluster(mapa(at + 2 * QT * 4, z));
           if (mz != -INFINITY || lz != 0.f) Lr += lz * ex2(mz - M);
         }
+        if (!Q8 && !in_range<PT>(Lr, M)) Lr = INFINITY;  // (computed again)
       }
       __syncwarp();
       cluster_sync();  // the parts have landed, and no CTA reads another's m and l any more

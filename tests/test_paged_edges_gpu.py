@@ -123,3 +123,17 @@ def test_bf16_queries_at_the_ends_of_their_range_over_int8_pages(torch, P, top, 
     x = x.bfloat16()
     s.pages[0].abs_().clamp_(min=1)
     check_attention(torch, s, x, s.cache.attention(x, s.batch))
+
+
+@pytest.mark.parametrize("dtype,top,size", [("f16", 65504, 2e4), ("f16", -65504, 2e4), ("f16", -65504, 300), ("f16", 6e3, 2e4)] +
+                         [("bf16", x * 2.0 ** e, 1) for x in (1, -1) for e in (24, 30, 100, 112, 119)])
+@pytest.mark.parametrize("q,kv", [([1], [50]), ([3, 1], [2100, 77]), ([30, 1], [99, 700]), ([300], [3000])])
+def test_scores_whose_last_bit_is_above_one(torch, P, dtype, top, size, q, kv):
+    """Scores of 2^24 and more, exact in f32 and all of one sign: their factor rounds by octaves,
+    and the key with the largest takes all."""
+    s = Setup(torch, P, q, kv, dtype, False, 32, 2)
+    x = torch.zeros((s.T, 8, D), device="cuda")
+    x[..., 3] = top
+    s.pages[0][..., 3] = (torch.rand(s.pages[0].shape[:3], generator=gen(torch, 6), device="cuda") * size + size / 8).to(s.pages[0].dtype)
+    x = x.to(s.pages[0].dtype)
+    check_attention(torch, s, x, s.cache.attention(x, s.batch))
