@@ -2215,8 +2215,11 @@ int64_t round_up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
 // ------------------------------------------------------------------ workspaces
 // GEMV workspace, independent of M and K so that one serves every linear of a
 // model: [partial-tile slots: 2 per resident warp][tile counters, zero between calls].
+// What follows it (a GGUF call's activations) must not lie on the counters of a linear with
+// more outputs that shares the workspace, so up to kSharedOutputs outputs its size is one.
 size_t gemv_workspace_bytes(int64_t N) {
-  const size_t cnt = (size_t)((N + 15) / 16) * sizeof(int);
+  constexpr int64_t kSharedOutputs = 262144;
+  const size_t cnt = (size_t)((std::max(N, kSharedOutputs) + 15) / 16) * sizeof(int);
   return (size_t)slot_bytes() + (size_t)round_up((int64_t)cnt, 256);
 }
 

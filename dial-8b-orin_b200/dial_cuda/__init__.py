@@ -161,7 +161,10 @@ def stream_ptr(stream=None) -> int:
 _stream_ws: dict = {}
 
 
-def stream_workspace(device, need: int):
+SHARED_OUTPUTS = 262144  # linears of more outputs do not share a workspace (their counters are longer)
+
+
+def stream_workspace(device, need: int, outputs: int = 0):
     """Zero-filled linear workspace shared by the calls issued on one stream.
 
     Calls on one stream run one after another, and every call leaves the
@@ -171,7 +174,8 @@ def stream_workspace(device, need: int):
     capture would come from the graph's private pool.
     """
     torch = _torch()
-    key = (device.index if device.index is not None else torch.cuda.current_device(), stream_ptr())
+    key = (device.index if device.index is not None else torch.cuda.current_device(), stream_ptr(),
+           outputs if outputs > SHARED_OUTPUTS else 0)
     ws = _stream_ws.get(key)
     if ws is None or ws.numel() < need:
         if torch.cuda.is_current_stream_capturing():
@@ -220,7 +224,8 @@ class W8A16Linear:
         rows = x.numel() // self.in_dim
         if out is None:
             out = torch.empty((*x.shape[:-1], self.out_dim), dtype=x.dtype, device=x.device)
-        ws, need = stream_workspace(x.device, lib().dial_w8a16_linear_workspace_bytes(self.out_dim))
+        ws, need = stream_workspace(x.device, lib().dial_w8a16_linear_workspace_bytes(self.out_dim),
+                                    self.out_dim)
         check(lib().dial_w8a16_linear(x.data_ptr(), dtype_code(x.dtype), self.qweight.data_ptr(),
                                       self.scales.data_ptr(), dtype_code(self.scales.dtype),
                                       out.data_ptr(), rows, self.in_dim, self.out_dim,
@@ -303,7 +308,7 @@ class GgufLinear:
     def workspace(self, rows: int):
         """Zero-filled workspace shared by the linears issued on the current stream."""
         need = lib().dial_gguf_linear_workspace_bytes(rows, self.in_dim, self.out_dim)
-        return stream_workspace(self.qs.device, need)
+        return stream_workspace(self.qs.device, need, self.out_dim)
 
     def forward(self, x, out=None):
         """x [..., in_dim] f32/f16/bf16 -> [..., out_dim] in x's dtype (worker_gguf.rs:574-611)."""

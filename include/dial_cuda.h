@@ -112,7 +112,7 @@ DIAL_API dial_status dial_w8a16_dequantize(const int8_t* q, const void* scale, d
  * zero-filled before its first use and every call leaves it zero-filled (a
  * call that reported a device error may not: zero it again).  Calls that share
  * a workspace must not overlap on the GPU.  One workspace sized for the largest
- * N serves every linear.  NULL: no workspace (same results, slower small M). */
+ * N serves every W8A16 linear.  NULL: no workspace (same results, slower small M). */
 DIAL_API size_t dial_w8a16_linear_workspace_bytes(int64_t N);
 DIAL_API dial_status dial_w8a16_linear(const void* x, dial_dtype xdt, const int8_t* q, const void* scale,
                               dial_dtype sdt, void* y, int64_t M, int64_t K, int64_t N,
@@ -165,7 +165,8 @@ DIAL_API dial_status dial_gguf_dequantize(const void* qs, const uint16_t* d, dia
  * dial_gguf_linear_workspace_bytes(M, K, N) bytes, 16-byte aligned, zero-filled
  * before its first use (every call leaves its counters zero again, unless it
  * reported a device error); calls that share a workspace must not overlap on
- * the GPU. */
+ * the GPU.  One workspace serves linears of up to 262144 outputs, W8A16 ones
+ * among them; a wider GGUF linear takes one of its own. */
 DIAL_API size_t dial_gguf_linear_workspace_bytes(int64_t M, int64_t K, int64_t N);
 DIAL_API dial_status dial_gguf_linear(const void* x, dial_dtype xdt, const void* qs, const uint16_t* d,
                              dial_ggml_type type, void* y, int64_t M, int64_t K, int64_t N,
