@@ -213,8 +213,13 @@ class W8A16Linear:
                                         stream_ptr()), "dial_w8a16_quantize")
         return cls(q, s, K, N, name)
 
-    def forward(self, x, out=None):
-        """x [..., in_dim] f16/bf16 -> [..., out_dim] same dtype (worker_w8a16.rs:368-386)."""
+    def workspace_bytes(self, rows: int) -> int:
+        return lib().dial_w8a16_linear_workspace_bytes(self.out_dim)
+
+    def forward(self, x, out=None, ws=None):
+        """x [..., in_dim] f16/bf16 -> [..., out_dim] same dtype (worker_w8a16.rs:368-386).
+        ws: a workspace of the caller's (uint8, zero-filled before its first use), instead of
+        the stream's."""
         torch = _torch()
         _require_cuda(x)
         if x.dtype not in (torch.float16, torch.bfloat16):
@@ -224,8 +229,11 @@ class W8A16Linear:
         rows = x.numel() // self.in_dim
         if out is None:
             out = torch.empty((*x.shape[:-1], self.out_dim), dtype=x.dtype, device=x.device)
-        ws, need = stream_workspace(x.device, lib().dial_w8a16_linear_workspace_bytes(self.out_dim),
-                                    self.out_dim)
+        need = self.workspace_bytes(rows)
+        if ws is None:
+            ws, need = stream_workspace(x.device, need, self.out_dim)
+        elif ws.numel() < need:
+            raise ValueError(f"W8A16 workspace must hold {need} bytes, got {ws.numel()}")
         check(lib().dial_w8a16_linear(x.data_ptr(), dtype_code(x.dtype), self.qweight.data_ptr(),
                                       self.scales.data_ptr(), dtype_code(self.scales.dtype),
                                       out.data_ptr(), rows, self.in_dim, self.out_dim,
@@ -305,13 +313,17 @@ class GgufLinear:
                                          stream_ptr()), "dial_gguf_dequantize")
         return w
 
+    def workspace_bytes(self, rows: int) -> int:
+        return lib().dial_gguf_linear_workspace_bytes(rows, self.in_dim, self.out_dim)
+
     def workspace(self, rows: int):
         """Zero-filled workspace shared by the linears issued on the current stream."""
-        need = lib().dial_gguf_linear_workspace_bytes(rows, self.in_dim, self.out_dim)
-        return stream_workspace(self.qs.device, need, self.out_dim)
+        return stream_workspace(self.qs.device, self.workspace_bytes(rows), self.out_dim)
 
-    def forward(self, x, out=None):
-        """x [..., in_dim] f32/f16/bf16 -> [..., out_dim] in x's dtype (worker_gguf.rs:574-611)."""
+    def forward(self, x, out=None, ws=None):
+        """x [..., in_dim] f32/f16/bf16 -> [..., out_dim] in x's dtype (worker_gguf.rs:574-611).
+        ws: a workspace of the caller's (uint8, zero-filled before its first use), instead of
+        the stream's."""
         torch = _torch()
         _require_cuda(x)
         if x.shape[-1] != self.in_dim:
@@ -319,7 +331,11 @@ class GgufLinear:
         rows = x.numel() // self.in_dim
         if out is None:
             out = torch.empty((*x.shape[:-1], self.out_dim), dtype=x.dtype, device=x.device)
-        ws, need = self.workspace(rows)
+        need = self.workspace_bytes(rows)
+        if ws is None:
+            ws, need = self.workspace(rows)
+        elif ws.numel() < need:
+            raise ValueError(f"GGUF workspace must hold {need} bytes, got {ws.numel()}")
         check(lib().dial_gguf_linear(x.data_ptr(), dtype_code(x.dtype), self.qs.data_ptr(),
                                      self.d.data_ptr(), self.qtype, out.data_ptr(), rows, self.in_dim,
                                      self.out_dim, ws.data_ptr() if need else None, need,

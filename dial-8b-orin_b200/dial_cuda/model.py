@@ -263,7 +263,12 @@ class Stage:
         `batch` (several sequences at once, prompt pieces or drafted tokens) are appended and
         attend their sequences' pages.  positions int32 [T] or [n_axes, T] with `sections`
         (`PagedKVCache.append`), tables: `rope_tables(rows, cfg.rope_theta)`.  Rows of hidden
-        behind the batch's last token come out unspecified."""
+        behind the batch's last token come out unspecified.  All memory is the call's own, so
+        calls and captured graphs may run on any streams, at once where their caches differ."""
+        with _torch().cuda.device(self.device):
+            return self._layers_paged(hidden, positions, batch, caches, tables, sections, interleaved)
+
+    def _layers_paged(self, hidden, positions, batch, caches, tables, sections, interleaved):
         torch = _torch()
         c, T = self.cfg, hidden.shape[0]
         _tensor(hidden, "hidden", self.dt, (T, c.hidden), max(hidden.get_device(), 0))
@@ -273,6 +278,8 @@ class Stage:
         qkv = torch.empty((T, (c.n_heads + 2 * c.n_kv_heads) * c.head_dim), dtype=self.dt, device=self.device)
         q, attn = (torch.zeros((T, c.n_heads, c.head_dim), dtype=self.dt, device=self.device) for _ in range(2))
         mid = torch.empty((T, c.intermediate), dtype=self.dt, device=self.device)
+        # one workspace for all linears: its counters are zeroed here and left zero by each
+        ws = torch.zeros(max((l.lin.workspace_bytes(T) for l in self.linears), default=0), dtype=torch.uint8, device=self.device)
 
         def norm(res, w):  # x = rms(hidden + res), hidden += res
             check(lib().dial_rmsnorm((hidden if res is None else res).data_ptr(), None if res is None else hidden.data_ptr(),
@@ -281,21 +288,25 @@ class Stage:
 
         for lin, norms, cache in zip(self.layer_linears, self.layer_norms, caches):
             norm(delta, norms["input_norm"])
-            lin["qkv"].lin.forward(x, qkv)
+            lin["qkv"].lin.forward(x, qkv, ws)
             cache.append(qkv, batch, *tables, positions, q_norm=norms["q_norm"] if c.qk_norm else None,
                          k_norm=norms["k_norm"] if c.qk_norm else None, eps=c.rms_eps, sections=sections,
                          interleaved=interleaved, out=q)
             cache.attention(q, batch, out=attn)
-            norm(lin["o"].lin.forward(attn.view(T, -1)), norms["post_norm"])
-            gate_up = lin["gate_up"].lin.forward(x)
+            norm(lin["o"].lin.forward(attn.view(T, -1), ws=ws), norms["post_norm"])
+            gate_up = lin["gate_up"].lin.forward(x, ws=ws)
             check(lib().dial_swiglu(gate_up.data_ptr(), mid.data_ptr(), dtype_code(self.dt), T, c.intermediate,
                                     stream_ptr()), "dial_swiglu")
-            delta = lin["down"].lin.forward(mid)
+            delta = lin["down"].lin.forward(mid, ws=ws)
         return hidden if delta is None else hidden.add_(delta)
 
-    def head_forward(self, hidden, out_ids, row_index=None, logits=None):
+    def head_forward(self, hidden, out_ids, row_index=None, logits=None, ws=None):
+        """ws: a workspace of the caller's (`head_workspace`) instead of the stage's."""
         rows = out_ids.numel()
-        ws, need = self.workspace(max(rows, hidden.shape[0]), 1)
+        if ws is None:
+            ws, need = self.workspace(max(rows, hidden.shape[0]), 1)
+        else:
+            need = ws.numel()
         check(self.L.dial_decoder_head(ctypes.byref(self.dims), self.final_norm.data_ptr(),
                                        self.head.ref, hidden.data_ptr(),
                                        row_index.data_ptr() if row_index is not None else None,
@@ -304,6 +315,14 @@ class Stage:
                                        ws.data_ptr(), need, stream_ptr()), "dial_decoder_head")
         return out_ids
 
+    def head_workspace(self, rows: int):
+        """A workspace for `head_forward` of `rows` rows, to be used by one call at a time."""
+        torch, c = _torch(), self.cfg
+        ws = torch.empty(self.L.dial_decoder_workspace_bytes(ctypes.byref(self.dims), rows, 1), dtype=torch.uint8, device=self.device)
+        # the counters at its start begin at zero; the rest is written before it is read
+        widest = max(c.vocab, 2 * c.intermediate, (c.n_heads + 2 * c.n_kv_heads) * c.head_dim, c.hidden)
+        ws[:self.L.dial_w8a16_linear_workspace_bytes(widest)].zero_()
+        return ws
 
     def head_shard_forward(self, hidden, keys_out, row_index=None, logits=None):
         """This stage's share of a vocabulary-parallel head: keys_out (int64
@@ -390,10 +409,11 @@ class Decoder:
         torch = _torch()
         st, T = self.stage, ids.numel()
         _tensor(ids, "ids", torch.int32, (T,), max(ids.get_device(), 0))
-        hidden = torch.empty((T, self.cfg.hidden), device=st.device, dtype=st.dt)
-        st.embed_tokens(ids, hidden)
-        st.layers_forward_paged(hidden, positions, batch, caches, tables, sections, interleaved)
-        logits = torch.empty((T, self.cfg.vocab), device=st.device, dtype=st.dt)
-        out = torch.empty(T, device=st.device, dtype=torch.int32)
-        st.head_forward(hidden, out, logits=logits)
+        with torch.cuda.device(st.device):
+            hidden = torch.empty((T, self.cfg.hidden), device=st.device, dtype=st.dt)
+            st.embed_tokens(ids, hidden)
+            st.layers_forward_paged(hidden, positions, batch, caches, tables, sections, interleaved)
+            logits = torch.empty((T, self.cfg.vocab), device=st.device, dtype=st.dt)
+            out = torch.empty(T, device=st.device, dtype=torch.int32)
+            st.head_forward(hidden, out, logits=logits, ws=st.head_workspace(T))
         return logits, out
