@@ -1,4 +1,6 @@
 // extern "C" entry points of the paged-cache operators (include/dial_cuda.h).
+#include <initializer_list>
+
 #include "common.cuh"
 #include "glue.cuh"
 #include "paged.cuh"
@@ -49,10 +51,45 @@ dial_status find_flag(int** err) {
   return *err ? DIAL_OK : fail(DIAL_ERR_CUDA, "device error flag unavailable");
 }
 
-// Whether [a, a + n) and [b, b + m) (bytes) share any.
-bool overlap(const void* a, int64_t n, const void* b, int64_t m) {
-  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
-  return x < y ? y - x < (uint64_t)n : x - y < (uint64_t)m;
+// An array of a call: `bytes` from `p` on (none if p is null).
+struct Span {
+  const char* name;
+  const void* p;
+  int64_t bytes;
+};
+
+bool overlap(const Span& a, const Span& b) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a.p), y = reinterpret_cast<uintptr_t>(b.p);
+  return a.p && b.p && (x < y ? y - x < (uint64_t)a.bytes : x - y < (uint64_t)b.bytes);
+}
+
+// What a call writes shares no memory with what it reads, nor with one another: its CTAs run in
+// any order.
+dial_status disjoint(std::initializer_list<Span> written, std::initializer_list<Span> read) {
+  for (const Span* w = written.begin(); w != written.end(); ++w) {
+    for (const Span* o = written.begin(); o != w; ++o)
+      if (overlap(*w, *o)) return fail(DIAL_ERR_INVALID_ARG, "%s must not overlap %s", w->name, o->name);
+    for (const Span& r : read)
+      if (overlap(*w, r)) return fail(DIAL_ERR_INVALID_ARG, "%s must not overlap %s", w->name, r.name);
+  }
+  return DIAL_OK;
+}
+
+struct KvSpans {
+  Span k, v, ks, vs;
+};
+KvSpans kv_spans(const dial_paged_kv* kv) {
+  const bool q8 = kv->format == DIAL_KV_INT8;
+  const int64_t rows = kv->n_pages * kv->n_kv_heads * kv->page_size, row = q8 ? 128 : 256;
+  return {{"k_pages", kv->k_pages, rows * row}, {"v_pages", kv->v_pages, rows * row},
+          {"k_scale", q8 ? kv->k_scale : nullptr, rows * 4}, {"v_scale", q8 ? kv->v_scale : nullptr, rows * 4}};
+}
+struct BatchSpans {
+  Span table, len, start;
+};
+BatchSpans batch_spans(const dial_paged_batch* b) {
+  return {{"block_table", b->block_table, b->n_seqs * b->max_pages * 4}, {"kv_len", b->kv_len, b->n_seqs * 4ll},
+          {"q_start", b->q_start, (b->n_seqs + 1ll) * 4}};
 }
 
 dial_status check_heads(int hq, int hkv) {
@@ -114,8 +151,13 @@ dial_status dial_paged_kv_append(const void* qkv, const void* q_norm_w, const vo
       !aligned16(cos_t) || !aligned16(sin_t))
     return fail(DIAL_ERR_MISALIGNED, "qkv, q_out, norm weights and tables must be 16-byte aligned");
   const int64_t row = 256 * tokens;  // of one head, bytes
-  if (overlap(qkv, row * (n_heads + 2 * p.hkv), q_out, row * n_heads))
-    return fail(DIAL_ERR_INVALID_ARG, "q_out must not overlap qkv");
+  const KvSpans c = kv_spans(kv);
+  const BatchSpans b = batch_spans(batch);
+  if ((s = disjoint({{"q_out", q_out, row * n_heads}, c.k, c.v, c.ks, c.vs},
+                    {{"qkv", qkv, row * (n_heads + 2 * p.hkv)}, {"q_norm_w", q_norm_w, 256}, {"k_norm_w", k_norm_w, 256},
+                     {"cos_t", cos_t, table_rows * 256}, {"sin_t", sin_t, table_rows * 256},
+                     {"positions", positions, 4 * tokens * r.n_axes}, b.table, b.len, b.start})) != DIAL_OK)
+    return s;
   if ((s = find_flag(&p.err)) != DIAL_OK) return s;
   return launch_paged_append(qkv, r, p, kv->format, q_out, dt, n_heads, as_stream(stream));
 }
@@ -129,8 +171,11 @@ dial_status dial_paged_kv_read(const dial_paged_kv* kv, const dial_paged_batch* 
   if (s != DIAL_OK) return s;
   if (!aligned16(k_out) || !aligned16(v_out))
     return fail(DIAL_ERR_MISALIGNED, "k_out and v_out must be 16-byte aligned");
-  if (overlap(k_out, 256 * tokens * p.hkv, v_out, 256 * tokens * p.hkv))
-    return fail(DIAL_ERR_INVALID_ARG, "k_out and v_out must not overlap");
+  const KvSpans c = kv_spans(kv);
+  const BatchSpans b = batch_spans(batch);
+  if ((s = disjoint({{"k_out", k_out, 256 * tokens * p.hkv}, {"v_out", v_out, 256 * tokens * p.hkv}},
+                    {c.k, c.v, c.ks, c.vs, b.table, b.len, b.start})) != DIAL_OK)
+    return s;
   if ((s = find_flag(&p.err)) != DIAL_OK) return s;
   return launch_paged_read(p, kv->format, k_out, v_out, dt, as_stream(stream));
 }
@@ -146,8 +191,11 @@ dial_status dial_paged_attention(const void* q, const dial_paged_kv* kv, const d
   if ((s = check_heads(n_heads, p.hkv)) != DIAL_OK) return s;
   if (!(scale > 0.f) || scale > 1e30f) return fail(DIAL_ERR_INVALID_ARG, "scale must be positive and finite");
   if (!aligned16(q) || !aligned16(out)) return fail(DIAL_ERR_MISALIGNED, "q and out must be 16-byte aligned");
-  if (overlap(q, 256 * tokens * n_heads, out, 256 * tokens * n_heads))
-    return fail(DIAL_ERR_INVALID_ARG, "out must not overlap q");
+  const KvSpans c = kv_spans(kv);
+  const BatchSpans b = batch_spans(batch);
+  if ((s = disjoint({{"out", out, 256 * tokens * n_heads}},
+                    {{"q", q, 256 * tokens * n_heads}, c.k, c.v, c.ks, c.vs, b.table, b.len, b.start})) != DIAL_OK)
+    return s;
   if ((s = find_flag(&p.err)) != DIAL_OK) return s;
   return launch_paged_attention(q, p, kv->format, out, dt, n_heads, batch->max_kv, scale, as_stream(stream));
 }
@@ -176,9 +224,17 @@ dial_status dial_verify_drafts(const void* logits, dial_dtype dt, const int32_t*
     return fail(DIAL_ERR_INVALID_ARG, "verification workspace must hold %zu bytes", need);
   if (!aligned16(logits) || !aligned16(draft_probs) || !aligned16(workspace))
     return fail(DIAL_ERR_MISALIGNED, "logits, draft_probs and workspace must be 16-byte aligned");
-  int* err = nullptr;
-  const dial_status s = find_flag(&err);
+  const int64_t cells = rows * vocab < (1ll << 60) ? rows * vocab : 1ll << 60;  // (no array is larger)
+  const int64_t e = dt == DIAL_F32 ? 4 : 2;
+  dial_status s = disjoint({{"out_ids", out_ids, 4 * rows}, {"n_out", n_out, 4ll * n_seqs}, {"logprobs", logprobs, 4 * rows},
+                            {"workspace", workspace, (int64_t)need}},
+                           {{"logits", logits, cells * e}, {"ids", ids, 4 * rows},
+                            {"draft_probs", draft_probs, cells * 4}, {"q_start", q_start, 4 * (n_seqs + 1ll)},
+                            {"temperature", temperature, 4ll * n_seqs}, {"accept_u", accept_u, 4 * rows},
+                            {"sample_u", sample_u, 4ll * n_seqs}});
   if (s != DIAL_OK) return s;
+  int* err = nullptr;
+  if ((s = find_flag(&err)) != DIAL_OK) return s;
   const VerifyArgs a{logits, ids, draft_probs, q_start, temperature, accept_u, sample_u, out_ids, n_out,
                      logprobs, err, rows, vocab, n_seqs, (int)(max_q < rows ? max_q : rows)};
   return launch_verify(a, dt, workspace, as_stream(stream));

@@ -470,8 +470,9 @@ typedef struct dial_rope_axes {
  * absmax / 127 (1 for a row below 1e-30) and code = round(x * (1 / scale)), halves
  * away from zero, as dial_w8a16_quantize; a row with a NaN or an infinity is kept
  * as NaN.  A position outside the table sets the device error flag and uses its
- * nearest row.  Two tokens of one call must not share a cache row; q_out must not
- * overlap qkv. */
+ * nearest row.  Two tokens of one call must not share a cache row.  Here and in the
+ * calls below, what a call writes must not overlap another of its arrays, or it is
+ * refused. */
 DIAL_API dial_status dial_paged_kv_append(
     const void* qkv, const void* q_norm_w, const void* k_norm_w, const float* cos_t,
     const float* sin_t, int64_t table_rows, const int32_t* positions, const dial_rope_axes* axes,
@@ -488,7 +489,7 @@ DIAL_API dial_status dial_paged_kv_read(const dial_paged_kv* kv, const dial_page
 /* Attention of the batch's tokens (q [T, Hq, 128] in dt) over the pages: token t
  * attends the cache rows up to its own, out [T, Hq * 128] =
  * softmax(scale * q.K^T) V.  Rows that a token does not attend do not touch its
- * result, whatever they hold.  Needs no workspace; out must not overlap q.  Where a
+ * result, whatever they hold.  Needs no workspace.  Where a
  * value row that is not finite, or an int8 row's scale that is 0 or below 2^-90, sits
  * near a token's rows, that token is computed key by key, which is far slower. */
 DIAL_API dial_status dial_paged_attention(const void* q, const dial_paged_kv* kv,
