@@ -1,43 +1,6 @@
 //! Rust binding of the B200 (sm_100a) kernels of DIAL's quantized-linear hot
 //! path: the `extern "C"` declarations of every entry point of
-//! `include/dial_cuda.h`, its `/// A paged KV cache: pages `[n_pages, n_kv_heads, page_size, 128]`.
-#[repr(C)]
-#[derive(Clone, Copy, Debug)]
-pub struct dial_paged_kv {
-    pub k_pages: *mut c_void,
-    pub v_pages: *mut c_void,
-    pub k_scale: *mut f32,
-    pub v_scale: *mut f32,
-    pub format: dial_kv_format,
-    pub n_kv_heads: i32,
-    pub head_dim: i32,
-    pub page_size: i32,
-    pub n_pages: i64,
-}
-
-/// Chunks of new tokens of several sequences over a paged cache.
-#[repr(C)]
-#[derive(Clone, Copy, Debug)]
-pub struct dial_paged_batch {
-    pub block_table: *const i32,
-    pub kv_len: *const i32,
-    pub q_start: *const i32,
-    pub n_seqs: i32,
-    pub max_pages: i64,
-    pub max_q: i64,
-    pub max_kv: i64,
-}
-
-/// Rotary positions with 1 to 4 axes.
-#[repr(C)]
-#[derive(Clone, Copy, Debug)]
-pub struct dial_rope_axes {
-    pub n_axes: i32,
-    pub section: [i32; 4],
-    pub interleaved: i32,
-}
-
-#[repr(C)]` structs, and a thin safe layer
+//! `include/dial_cuda.h`, its `#[repr(C)]` structs, and a thin safe layer
 //! (status codes to `Result`).
 //!
 //! The reference's host side sits behind candle's `CustomOp1`
@@ -229,6 +192,43 @@ pub struct dial_plan_result {
     pub states_considered: i64,
     pub feasible_transitions: i64,
     pub rejected_for_memory: i64,
+}
+
+/// A paged KV cache: pages `[n_pages, n_kv_heads, page_size, 128]`.
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct dial_paged_kv {
+    pub k_pages: *mut c_void,
+    pub v_pages: *mut c_void,
+    pub k_scale: *mut f32,
+    pub v_scale: *mut f32,
+    pub format: dial_kv_format,
+    pub n_kv_heads: i32,
+    pub head_dim: i32,
+    pub page_size: i32,
+    pub n_pages: i64,
+}
+
+/// Chunks of new tokens of several sequences over a paged cache.
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct dial_paged_batch {
+    pub block_table: *const i32,
+    pub kv_len: *const i32,
+    pub q_start: *const i32,
+    pub n_seqs: i32,
+    pub max_pages: i64,
+    pub max_q: i64,
+    pub max_kv: i64,
+}
+
+/// Rotary positions with 1 to 4 axes.
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct dial_rope_axes {
+    pub n_axes: i32,
+    pub section: [i32; 4],
+    pub interleaved: i32,
 }
 
 /// Opaque NCCL stage communicator (one pipeline link).
