@@ -137,3 +137,31 @@ def test_scores_whose_last_bit_is_above_one(torch, P, dtype, top, size, q, kv):
     s.pages[0][..., 3] = (torch.rand(s.pages[0].shape[:3], generator=gen(torch, 6), device="cuda") * size + size / 8).to(s.pages[0].dtype)
     x = x.to(s.pages[0].dtype)
     check_attention(torch, s, x, s.cache.attention(x, s.batch))
+
+
+@pytest.mark.parametrize("q,kv", [([6], [300]), ([70, 40], [300, 141]), ([1], [4000])])
+@pytest.mark.parametrize("dtype,quant,bad,whole", [("bf16", False, b, w) for b in (math.nan, math.inf, -math.inf) for w in (True, False)] +
+                         [("f16", False, b, False) for b in (math.nan, math.inf, -math.inf)] +
+                         [("bf16", True, math.nan, True), ("f16", True, math.nan, True)])
+@pytest.mark.parametrize("back", [1, 2, 3, 6, 150])
+def test_a_key_that_is_not_finite(torch, P, q, kv, dtype, quant, bad, whole, back):
+    """One key row, or one value of it, of kv head 0: tokens that see it have what the definition
+    gives them, NaN or what the other keys give, the others nothing of it."""
+    s = Setup(torch, P, q, kv, dtype, quant, 64, 2)
+    at = kv[0] - back
+    page, row = s.host_table[0][at // 64], at % 64
+    if quant:
+        s.scales[0][page, 0, row] = bad
+    else:
+        s.pages[0][page, 0, row, slice(None) if whole else 9] = bad
+    x = torch.randn((s.T, 8, D), generator=gen(torch, 4), device="cuda").to(dtype_of(torch, dtype))
+    got = s.cache.attention(x, s.batch)
+    want, size = attention64(torch, s, x, D ** -0.5)
+    nan = torch.isnan(want)
+    sees = torch.zeros(got.shape[:2], dtype=torch.bool, device="cuda")
+    sees[max(0, q[0] - back):q[0], :4] = True
+    assert not nan[~sees].any() and (nan[sees].all() if whole else True)
+    assert torch.equal(torch.isnan(got), nan)
+    u = torch.finfo(x.dtype).eps / 2
+    off = (got.double() - want).abs()
+    assert torch.all((off <= u * want.abs() + (u + 2.0 ** -12) * size + 1e-7) | nan)

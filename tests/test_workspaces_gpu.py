@@ -177,3 +177,22 @@ def test_captured_paged_steps_keep_their_memory(torch, lib, name):
         for o, w in zip(outs, want):
             assert torch.equal(o, w)
     assert all(bool((t == 0x5A).all()) for t in taken)
+
+
+@pytest.mark.parametrize("quantized", [False, True])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_forward_paged_with_several_axes(torch, lib, quantized, interleaved):
+    """Three axes at the same positions are one axis, bit for bit; at others they are not."""
+    p = Paged(torch, "w8a16")
+    out = []
+    for axes in (1, 3):
+        s = p.state(6, quantized)
+        p.chunk(s, 40, 50)
+        ids, pos, batch, caches = s.args
+        if axes == 1:
+            out.append(p.call(s.args)[0])
+        else:
+            kw = dict(sections=(24, 20, 20), interleaved=interleaved)
+            out.append(p.call((ids, pos.expand(3, -1).contiguous(), batch, caches), **kw)[0])
+            out.append(p.call((ids, torch.stack([pos, pos + 3, pos // 2]).contiguous(), batch, caches), **kw)[0])
+    assert torch.equal(out[0], out[1]) and not torch.equal(out[0], out[2])
