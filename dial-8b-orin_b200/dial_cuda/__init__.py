@@ -159,6 +159,7 @@ def stream_ptr(stream=None) -> int:
 
 
 _stream_ws: dict = {}
+_captured_ws: dict = {}  # workspaces that a captured graph writes to, kept alive: address -> tensor
 
 
 SHARED_OUTPUTS = 262144  # linears of more outputs do not share a workspace (their counters are longer)
@@ -171,7 +172,8 @@ def stream_workspace(device, need: int, outputs: int = 0):
     workspace's counters zero, so they can share it; another stream gets its own.
     A stream that is being captured into a CUDA graph must have its workspace
     already (one eager call on that stream first): an allocation inside the
-    capture would come from the graph's private pool.
+    capture would come from the graph's private pool.  A workspace that a capture
+    has used stays allocated when a larger one takes its place.
     """
     torch = _torch()
     key = (device.index if device.index is not None else torch.cuda.current_device(), stream_ptr(),
@@ -183,6 +185,8 @@ def stream_workspace(device, need: int, outputs: int = 0):
                                "eager call on that stream before capturing")
         ws = torch.zeros(max(need, 256), dtype=torch.uint8, device=device)
         _stream_ws[key] = ws
+    elif torch.cuda.is_current_stream_capturing():
+        _captured_ws[ws.data_ptr()] = ws
     return ws, need
 
 

@@ -213,6 +213,7 @@ class Stage:
         check(self.L.dial_rope_tables(self.cos.data_ptr(), self.sin.data_ptr(), dtype_code(self.dt),
                                       max_seq, D, c.rope_theta, stream_ptr()), "dial_rope_tables")
         self._ws = None
+        self._captured_ws = {}  # workspaces that a captured graph writes to, kept alive: address -> tensor
         torch.cuda.synchronize(self.device)
 
     # -------------------------------------------------------------- sizes
@@ -228,9 +229,15 @@ class Stage:
     def workspace(self, tokens: int, max_len: int):
         torch = _torch()
         need = self.L.dial_decoder_workspace_bytes(ctypes.byref(self.dims), tokens, max_len)
+        capturing = torch.cuda.is_current_stream_capturing()
         if self._ws is None or self._ws.numel() < need:
             # zero-filled: the stream-K counters at its start must begin at zero
-            self._ws = torch.zeros(need, dtype=torch.uint8, device=self.device)
+            ws = torch.zeros(need, dtype=torch.uint8, device=self.device)
+            if capturing:
+                return ws, need  # the graph's own, zeroed by its replays and not before
+            self._ws = ws
+        if capturing:
+            self._captured_ws[self._ws.data_ptr()] = self._ws
         return self._ws, need
 
     # -------------------------------------------------------------- forward pieces

@@ -196,3 +196,62 @@ def test_forward_paged_with_several_axes(torch, lib, quantized, interleaved):
             out.append(p.call((ids, pos.expand(3, -1).contiguous(), batch, caches), **kw)[0])
             out.append(p.call((ids, torch.stack([pos, pos + 3, pos // 2]).contiguous(), batch, caches), **kw)[0])
     assert torch.equal(out[0], out[1]) and not torch.equal(out[0], out[2])
+
+
+# ------------------------------------------------------------------ graphs over the shared workspaces
+def fill(torch):
+    """Free blocks of the allocator, taken and filled."""
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    return [torch.full((n,), 0x5A, dtype=torch.uint8, device="cuda") for n in [1 << 20] * 40 + [1 << 24] * 10]
+
+
+@pytest.mark.parametrize("eager_first", [True, False])
+def test_a_captured_decode_step_after_a_larger_prefill(torch, lib, eager_first):
+    """The stage's workspace grows behind a captured step, or is first asked for by one."""
+    from dial_cuda.model import Decoder, ModelConfig
+    dec = Decoder(ModelConfig(**CONFIGS["w8a16"]), n_slots=2, max_seq=256)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    ids, pos, slot, out = torch.tensor([7], **i32), torch.tensor([0], **i32), torch.tensor([1], **i32), torch.empty(1, **i32)
+    hidden = torch.empty((1, dec.cfg.hidden), device="cuda", dtype=dec.stage.dt)
+    if eager_first:
+        dec.decode_step(ids, pos, slot, 1, out, hidden=hidden)
+    gr = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(gr):
+        dec.decode_step(ids, pos, slot, 1, out, hidden=hidden)
+    prompt = torch.arange(200, **i32)
+    first = dec.prefill(prompt, slot=0)
+    assert torch.equal(dec.prefill(prompt, slot=0), first)
+    taken = fill(torch)
+    for _ in range(3):
+        gr.replay()
+        assert torch.equal(dec.prefill(prompt, slot=0), first)
+    torch.cuda.synchronize()
+    got, bits = out.clone(), hidden.clone()
+    dec.decode_step(ids, pos, slot, 1, out, hidden=hidden)
+    assert torch.equal(out, got) and torch.equal(hidden, bits)
+    assert all(bool((t == 0x5A).all()) for t in taken)
+
+
+def test_a_captured_linear_after_a_larger_call(torch, lib):
+    g = gen(torch, 8)
+    lin = lib.GgufLinear.quantize(torch.randn((512, 1152), generator=g, device="cuda") * 0.05, lib.Q4_0)
+    x, big = (torch.randn((m, 1152), generator=g, device="cuda").half() for m in (9, 3000))
+    side, gr = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    out = torch.empty((9, 512), device="cuda", dtype=torch.float16)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        want = lin.forward(x)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(gr, stream=side):
+        lin.forward(x, out)
+    with torch.cuda.stream(side):
+        lin.forward(big)
+    taken = fill(torch)
+    for _ in range(3):
+        out.zero_()
+        gr.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+    assert all(bool((t == 0x5A).all()) for t in taken)
