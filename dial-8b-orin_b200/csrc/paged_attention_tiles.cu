@@ -25,10 +25,11 @@
 // Few rows and many keys: the key tiles are split over a cluster of CTAs, whose
 // (m, l, O) meet in distributed shared memory, so that no workspace is needed
 // and the result does not depend on timing.
-// 2048 tokens of 32 heads behind 14336 others in bf16 take 422 us, 1.22 PFLOP/s; inside a
-// CTA a key tile of 2 x 128 rows takes 1.7 us, in which the tensor cores and the exponentials
-// are busy alike (64 %), and 256 CTAs are 1.73 rounds over the SMs.  8 ragged int8 chunks of up to
-// 777 tokens take 99.5 us, 0.61 PFLOP/s: widening the codes shares the shared memory's
+// 2048 tokens of 32 heads behind 14336 others in bf16 take 422 us, 1.22 PFLOP/s, at 1965 MHz
+// (490, 1.05, once the power limit has lowered the clock); inside a CTA a key tile of 2 x 128
+// rows takes 1.7 us, in which the tensor cores and the exponentials are busy alike (65 %), and
+// 256 CTAs are 1.73 rounds over the SMs.  8 ragged int8 chunks of up to 777 tokens take 99.5
+// us, 0.61 PFLOP/s (99 to 114 from run to run): widening the codes shares the shared memory's
 // bandwidth with the MMAs' operands.
 // Every mbarrier wait is bounded (1 s), flags DIAL_ERR_TIMEOUT and gives up.
 #include <cuda.h>
@@ -531,6 +532,7 @@ __global__ void __launch_bounds__(Cfg<Q8>::THREADS, 1)
               y = fma2(make_float2(s[e + 2], s[e + 3]), make_float2(a.c, a.c), make_float2(sub, sub));
             }
             x.x = ex2(x.x), x.y = ex2(x.y), y.x = ex2(y.x), y.y = ex2(y.y);
+            // (rounded to the operands' type, as paged_attention.cu does)
             pk[(e & 63) / 2] = pack2<PT>(x.x, x.y);
             pk[(e & 63) / 2 + 1] = pack2<PT>(y.x, y.y);
             if constexpr (Q8) {

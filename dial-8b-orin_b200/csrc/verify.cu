@@ -16,8 +16,10 @@
 //      value: every warp a run of the row, then the one run that the number falls in
 //      once more, element by element.
 // 32 sequences of up to 6 rows of 151936 in bf16 with the drafts' probabilities (47 MB)
-// take 32.7 us, 9.5 of them the segments, about 12 the f64 sweep; one sequence of 4 rows
-// takes 13.0 us, the chain of its steps.
+// take 33 us, 9.5 of them the segments; one sequence of 4 rows takes 13.2 us, the chain of
+// its steps.  The f64 pipe is busy 18 % of the draw, and with f32 exponents in its sweep the
+// 32 took 0.7 us less: what binds it is the waiting from step to step (segments, acceptance,
+// row, one to two meetings of the cluster, the run again), barriers before loads.
 #include <algorithm>
 
 #include "common.cuh"
@@ -31,7 +33,12 @@ constexpr int SEG = 1024;           // a warp's piece of a row
 constexpr int kStatWarps = 4;
 constexpr int kDrawThreads = 512;
 constexpr int kWarps = kDrawThreads / 32;
-constexpr int HOLD = 5;             // vectors that a thread of the draw keeps
+// Vectors that a thread of the draw keeps: the least that holds a warp's run of 151936 16-bit
+// logits over eight CTAs (149 of 160).  Longer runs go by in pieces, and the drawn one is
+// loaded again: 32 sequences of 2 rows with probabilities take 29 us at 163800 16-bit logits
+// and 38 at 165000, 43 with 151936 in f32, and 52 us are 38 sequences (four CTAs each)
+// where 37 take 40.  With six, two CTAs of 112 KB and their static arrays no longer fit an SM.
+constexpr int HOLD = 5;
 constexpr int kDrawSmem = HOLD * kDrawThreads * 32 + 64 * 32 * 8;
 
 struct __align__(16) SegStat {

@@ -447,7 +447,9 @@ typedef struct dial_paged_batch {
   const int32_t* q_start;     /* [n_seqs + 1] */
   int32_t n_seqs;
   int64_t max_pages;
-  int64_t max_q;  /* no chunk is longer */
+  int64_t max_q;  /* no chunk is longer.  Up to max_q * (Hq / Hkv) = 32 rows attention takes
+                     the kernel for few rows; single tokens under a larger bound run as
+                     chunks (32 over 2049 int8 rows: 88 us instead of 33) */
   int64_t max_kv; /* the longest kv_len expected (sizes the key split only) */
 } dial_paged_batch;
 
@@ -489,7 +491,11 @@ DIAL_API dial_status dial_paged_kv_read(const dial_paged_kv* kv, const dial_page
 /* Attention of the batch's tokens (q [T, Hq, 128] in dt) over the pages: token t
  * attends the cache rows up to its own, out [T, Hq * 128] =
  * softmax(scale * q.K^T) V.  Rows that a token does not attend do not touch its
- * result, whatever they hold.  Needs no workspace.  Where a
+ * result, whatever they hold.  Scores, sums and maxima are f32; a probability is
+ * rounded once to the operands' type (f16, or dt over bf16 pages) before it meets the
+ * values, its sum is of the unrounded ones.  In f16 it keeps 11 bits down to 2^-21 of
+ * the row's largest (times its value scale over int8 pages, 1 for a row of zeros), and
+ * below 2^-32 it is zero.  Needs no workspace.  Where a
  * value row that is not finite, or an int8 row's scale that is 0 or below 2^-90, sits
  * near a token's rows, that token is computed key by key, which is far slower. */
 DIAL_API dial_status dial_paged_attention(const void* q, const dial_paged_kv* kv,
