@@ -19,7 +19,7 @@ import hashlib
 from dataclasses import dataclass, field
 from typing import Optional
 
-from . import (BF16, F16, F32, GgufLinear, W8A16Linear, _torch, check, dtype_code, lib,
+from . import (BF16, F16, F32, SHARED_OUTPUTS, GgufLinear, W8A16Linear, _torch, check, dtype_code, lib,
                stream_ptr)
 from .paged import PagedKVCache, _tensor
 
@@ -278,7 +278,7 @@ class Stage:
     def _layers_paged(self, hidden, positions, batch, caches, tables, sections, interleaved):
         torch = _torch()
         c, T = self.cfg, hidden.shape[0]
-        _tensor(hidden, "hidden", self.dt, (T, c.hidden), max(hidden.get_device(), 0))
+        _tensor(hidden, "hidden", self.dt, (T, c.hidden), self.cos.get_device())
         if len(caches) != self.last - self.first:
             raise ValueError(f"{self.last - self.first} layers take as many caches, got {len(caches)}")
         x, delta = torch.empty_like(hidden), None
@@ -286,7 +286,12 @@ class Stage:
         q, attn = (torch.zeros((T, c.n_heads, c.head_dim), dtype=self.dt, device=self.device) for _ in range(2))
         mid = torch.empty((T, c.intermediate), dtype=self.dt, device=self.device)
         # one workspace for all linears: its counters are zeroed here and left zero by each
-        ws = torch.zeros(max((l.lin.workspace_bytes(T) for l in self.linears), default=0), dtype=torch.uint8, device=self.device)
+        zeros = lambda n: torch.zeros(n, dtype=torch.uint8, device=self.device)
+        ws = zeros(max((l.lin.workspace_bytes(T) for l in self.linears), default=0))
+
+        def linear(l, x, out=None):
+            own = l.lin.out_dim > SHARED_OUTPUTS
+            return l.lin.forward(x, out, zeros(l.lin.workspace_bytes(T)) if own else ws)
 
         def norm(res, w):  # x = rms(hidden + res), hidden += res
             check(lib().dial_rmsnorm((hidden if res is None else res).data_ptr(), None if res is None else hidden.data_ptr(),
@@ -295,16 +300,16 @@ class Stage:
 
         for lin, norms, cache in zip(self.layer_linears, self.layer_norms, caches):
             norm(delta, norms["input_norm"])
-            lin["qkv"].lin.forward(x, qkv, ws)
+            linear(lin["qkv"], x, qkv)
             cache.append(qkv, batch, *tables, positions, q_norm=norms["q_norm"] if c.qk_norm else None,
                          k_norm=norms["k_norm"] if c.qk_norm else None, eps=c.rms_eps, sections=sections,
                          interleaved=interleaved, out=q)
             cache.attention(q, batch, out=attn)
-            norm(lin["o"].lin.forward(attn.view(T, -1), ws=ws), norms["post_norm"])
-            gate_up = lin["gate_up"].lin.forward(x, ws=ws)
+            norm(linear(lin["o"], attn.view(T, -1)), norms["post_norm"])
+            gate_up = linear(lin["gate_up"], x)
             check(lib().dial_swiglu(gate_up.data_ptr(), mid.data_ptr(), dtype_code(self.dt), T, c.intermediate,
                                     stream_ptr()), "dial_swiglu")
-            delta = lin["down"].lin.forward(mid, ws=ws)
+            delta = linear(lin["down"], mid)
         return hidden if delta is None else hidden.add_(delta)
 
     def head_forward(self, hidden, out_ids, row_index=None, logits=None, ws=None):
@@ -415,7 +420,7 @@ class Decoder:
         what `verify_drafts` takes, with the same ids and `batch.q_start`."""
         torch = _torch()
         st, T = self.stage, ids.numel()
-        _tensor(ids, "ids", torch.int32, (T,), max(ids.get_device(), 0))
+        _tensor(ids, "ids", torch.int32, (T,), st.cos.get_device())
         with torch.cuda.device(st.device):
             hidden = torch.empty((T, self.cfg.hidden), device=st.device, dtype=st.dt)
             st.embed_tokens(ids, hidden)

@@ -255,3 +255,18 @@ def test_a_captured_linear_after_a_larger_call(torch, lib):
         torch.cuda.synchronize()
         assert torch.equal(out, want)
     assert all(bool((t == 0x5A).all()) for t in taken)
+
+
+def test_forward_paged_with_a_linear_wider_than_a_shared_workspace_serves(torch, lib):
+    """gate_up of 262784 outputs: its counters are longer than the shared ones."""
+    CONFIGS["wide"] = dict(n_layers=2, hidden=384, intermediate=131392, n_heads=1, n_kv_heads=1, vocab=100, qk_norm=False,
+                           weight_format=8, head_format=8)
+    try:
+        p = Paged(torch, "wide")
+    finally:
+        del CONFIGS["wide"]
+    s = p.state(7)
+    first = p.chunk(s, 40, 42)[0]
+    assert torch.isfinite(first).all()
+    for _ in range(3):
+        assert torch.equal(p.call(s.args)[0], first)
